@@ -63,8 +63,10 @@ int y5_device_arch(char* buf, int n);
  * ------------------------------------------------------------------------------------------ */
 #define Y5_ACT_NONE 0
 #define Y5_ACT_LEAKY 1
+#define Y5_ACT_SILU 2 /* v / (1 + exp(-v)): group norm and the 8-bit product only */
 #define Y5_F16 0
 #define Y5_BF16 1
+#define Y5_F32 2 /* group norm and the 8-bit entry points only */
 
 typedef struct y5_conv_desc {
     const void* x;      /* input  (batch, h, w, cin) fp16, pixel pitch x_ld                         */
@@ -413,6 +415,76 @@ int y5_scale_coords_f32(float* det, const int32_t* count, const float* params, i
 int y5_nms_boxes_f32(const float* boxes, const float* scores, int n, double iou_thres, int64_t* keep,
                      int32_t* keep_count, int max_keep, void* workspace, size_t workspace_bytes,
                      y5_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Group norm with an activation, channels last, and its gradient.  No counterpart in the reference, whose blocks carry
+ * BatchNorm2d (models/common.py:27): the normalisation for batches too small for batch statistics.
+ *   mean, var: over the pixels and the c / groups channels of a group of one image (var biased, 32-bit sums of differences
+ *   from a value near the mean);  xh = (x - mean) / sqrt(var + eps);  z = xh * weight[c] + bias[c];  y = act(z), rounded once.
+ * Tensors are (batch, pixels, c) with pixel pitch *_ld and images pixels * ld apart.  Any channel count c that the groups
+ * divide; a pitch above c needs c in whole 16-byte vectors (multiples of 8, fp32: 4).  Pointers at element alignment.
+ * Limit: c * (V / gcd(c, V)) <= 4096 with V = 8 (fp32: 4) values of a 16-byte vector.
+ * y may be x; dx may be dy or x.  A group with an infinity or a NaN gives NaN throughout, other groups are untouched by it.
+ * Sums are taken in a fixed order: the same call gives the same bits.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct y5_group_norm_desc {
+    const void* x;      /* input */
+    void* y;            /* output (forward) */
+    const void* dy;     /* gradient of y (backward) */
+    void* dx;           /* gradient of x, or NULL = not wanted (backward) */
+    const void* weight; /* [c] of param_dtype, or NULL = ones */
+    const void* bias;   /* [c] of param_dtype, or NULL = zeros */
+    void* dweight;      /* [c] of param_dtype, or NULL = not wanted (backward) */
+    void* dbias;
+    float* mean;        /* [batch][groups]: written by the forward (both or neither), read by the backward */
+    float* rstd;        /* 1 / sqrt(var + eps) */
+    void* workspace;    /* y5_group_norm_workspace bytes, 16-byte aligned, used until the call's work on the stream is done */
+    size_t workspace_bytes;
+    int32_t batch, pixels, c, groups;
+    int32_t x_ld, y_ld, dy_ld, dx_ld;
+    int32_t dtype, param_dtype; /* Y5_F16, Y5_BF16, Y5_F32 */
+    int32_t act;                /* Y5_ACT_NONE, Y5_ACT_LEAKY, Y5_ACT_SILU */
+    float slope, eps;
+} y5_group_norm_desc;
+#define Y5_GN_FORWARD 0
+#define Y5_GN_BACKWARD 1
+#define Y5_GN_ROWS 2
+/* Workspace bytes of a call on the descriptor's shape (pointers and pitches are not looked at): what = Y5_GN_*.  May be 0. */
+int y5_group_norm_workspace(const y5_group_norm_desc* d, int what, size_t* bytes);
+int y5_group_norm(const y5_group_norm_desc* d, y5_stream_t stream);
+int y5_group_norm_backward(const y5_group_norm_desc* d, y5_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * 8-bit integers: rows with a scale each, and their product with a weight matrix with a scale a channel.  No counterpart in
+ * the reference; the 8-bit form of its 1x1 convolutions (models/common.py:26, :51-53) and linear layers, pixels as rows.
+ *   rows:    a = max |x| of a row, scale = a / 127, q = the whole number nearest to 127 x / a (computed in fp32 for 16-bit
+ *            inputs, in fp64 for fp32 ones).  a < 2^-120: scale 0 and zeros.  An infinity or a NaN in the row: scale NaN and
+ *            zeros.
+ *   product: y[m][n] = act( (sum_k a[m][k] w[n][k]) * (a_scale[m] * w_scale[n]) + bias[n] ), the sum exact in int32, the rest
+ *            in fp32, rounded once to dtype.
+ * A row of a or w is (k + 15) / 16 * 16 bytes, zeros behind the k-th, 16-byte aligned; q values lie in [-127, 127] (-128 is
+ * taken too).
+ * ------------------------------------------------------------------------------------------ */
+#define Y5_I8_MAX_K 131056 /* so many products of at most 2^14 stay below 2^31 */
+/* x: rows of k values of dtype at pitch x_ld; q: [rows][q_ld] with q_ld = (k + 15) / 16 * 16; scale: [rows] */
+int y5_quantize_rows_i8(const void* x, int64_t x_ld, int dtype, int64_t rows, int k, void* q, int q_ld, float* scale, y5_stream_t stream);
+/* Group norm + activation straight to 8-bit rows, one row a pixel: quantises the unrounded fp32 values of y5_group_norm.
+ * Descriptor as there; y, dy, dx, dweight, dbias, mean and rstd are not used. */
+int y5_group_norm_rows_i8(const y5_group_norm_desc* d, void* q, int q_ld, float* scale, y5_stream_t stream);
+typedef struct y5_gemm_i8_desc {
+    const void* a;        /* int8 [m][ld] */
+    const float* a_scale; /* [m] */
+    const void* w;        /* int8 [n][ld] */
+    const float* w_scale; /* [n] */
+    const float* bias;    /* [n] or NULL */
+    void* y;              /* [m] rows of n values of dtype at pitch y_ld, at element alignment */
+    int64_t m, y_ld;
+    int32_t n, k, ld;     /* ld = (k + 15) / 16 * 16 */
+    int32_t dtype;        /* Y5_F16, Y5_BF16, Y5_F32 */
+    int32_t act;          /* Y5_ACT_NONE, Y5_ACT_LEAKY, Y5_ACT_SILU */
+    float slope;
+} y5_gemm_i8_desc;
+int y5_gemm_i8(const y5_gemm_i8_desc* d, y5_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * Launch plans: a host-side list of the calls above, replayed with one C call per forward.

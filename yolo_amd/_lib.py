@@ -14,8 +14,10 @@ Y5_MAX_LEVELS = 4
 NMS_NOALLOC_BYTES = (16 << 20) + 4096  # Y5_NMS_NOALLOC_BYTES
 PLAN_SIDE, PLAN_JOIN = 1, 2
 NMS_AGNOSTIC, NMS_MERGE = 1, 2  # flags of y5_nms_desc.agnostic
-ACT_NONE, ACT_LEAKY = 0, 1
-F16, BF16 = 0, 1  # y5_conv_desc.dtype / y5_decode_desc.dtype
+ACT_NONE, ACT_LEAKY, ACT_SILU = 0, 1, 2
+F16, BF16, F32 = 0, 1, 2  # y5_conv_desc.dtype / y5_decode_desc.dtype; F32: group norm and the 8-bit entry points only
+GN_FORWARD, GN_BACKWARD, GN_ROWS = 0, 1, 2
+I8_MAX_K = 131056  # Y5_I8_MAX_K
 IN_F16, IN_U8, IN_U8_HWC, IN_U8_HWC_BGR = 0, 1, 2, 3  # input layouts of y5_focus_conv_u8_hwc
 OK, EINVAL, EHIP, ENOMEM, EWORKSPACE = 0, -1, -2, -3, -4  # y5_status in include/y5hip.h
 OP_NAMES = {19: 'focus_conv', 18: 'focus_conv', 17: 'conv', 16: 'conv', 14: 'focus_conv', 15: 'focus_conv', 13: 'conv', 12: 'detect', 8: 'focus_conv', 9: 'decode', 10: 'focus_conv', 11: 'normalize', 1: 'conv', 2: 'pack', 3: 'maxpool', 4: 'upsample', 5: 'copy', 6: 'decode', 7: 'maxpool'}
@@ -59,6 +61,21 @@ class NmsDesc(C.Structure):
                 ('agnostic', C.c_int32), ('max_candidates', C.c_int32), ('max_det', C.c_int32)]
 
 
+class GroupNormDesc(C.Structure):
+    _fields_ = [('x', C.c_void_p), ('y', C.c_void_p), ('dy', C.c_void_p), ('dx', C.c_void_p), ('weight', C.c_void_p),
+                ('bias', C.c_void_p), ('dweight', C.c_void_p), ('dbias', C.c_void_p), ('mean', C.c_void_p), ('rstd', C.c_void_p),
+                ('workspace', C.c_void_p), ('workspace_bytes', C.c_size_t),
+                ('batch', C.c_int32), ('pixels', C.c_int32), ('c', C.c_int32), ('groups', C.c_int32),
+                ('x_ld', C.c_int32), ('y_ld', C.c_int32), ('dy_ld', C.c_int32), ('dx_ld', C.c_int32),
+                ('dtype', C.c_int32), ('param_dtype', C.c_int32), ('act', C.c_int32), ('slope', C.c_float), ('eps', C.c_float)]
+
+
+class GemmI8Desc(C.Structure):
+    _fields_ = [('a', C.c_void_p), ('a_scale', C.c_void_p), ('w', C.c_void_p), ('w_scale', C.c_void_p), ('bias', C.c_void_p),
+                ('y', C.c_void_p), ('m', C.c_int64), ('y_ld', C.c_int64), ('n', C.c_int32), ('k', C.c_int32), ('ld', C.c_int32),
+                ('dtype', C.c_int32), ('act', C.c_int32), ('slope', C.c_float)]
+
+
 # name -> (restype, argtypes); every symbol include/y5hip.h declares
 _i, _p, _s = C.c_int, C.c_void_p, C.c_void_p
 SIGNATURES = {
@@ -93,6 +110,12 @@ SIGNATURES = {
     'y5_bn_stats_f16': (_i, [_p, _i, C.c_int64, _i, _p, _s]),
     'y5_bn_finalize_f32': (_i, [_p, _i, C.c_int64, _i, _i, _p, _p, C.c_float, C.c_float, _p, _p, _p, _p, _s]),
     'y5_affine_act_f16': (_i, [_p, _i, _p, _i, _p, _i, C.c_int64, _i, _p, _p, _i, C.c_float, _s]),
+    'y5_group_norm_workspace': (_i, [C.POINTER(GroupNormDesc), _i, C.POINTER(C.c_size_t)]),
+    'y5_group_norm': (_i, [C.POINTER(GroupNormDesc), _s]),
+    'y5_group_norm_backward': (_i, [C.POINTER(GroupNormDesc), _s]),
+    'y5_group_norm_rows_i8': (_i, [C.POINTER(GroupNormDesc), _p, _i, _p, _s]),
+    'y5_quantize_rows_i8': (_i, [_p, C.c_int64, _i, C.c_int64, _i, _p, _i, _p, _s]),
+    'y5_gemm_i8': (_i, [C.POINTER(GemmI8Desc), _s]),
     'y5_detect_decode_f16': (_i, [C.POINTER(DecodeDesc), _s]),
     'y5_detect_decode_multi_f16': (_i, [C.POINTER(DecodeDesc), C.c_int, _s]),
     'y5_detect_f16': (_i, [C.POINTER(ConvDesc), C.POINTER(DecodeDesc), C.c_int, _s]),

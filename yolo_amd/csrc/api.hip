@@ -106,6 +106,30 @@ extern "C" int y5_upsample2x_f16(const void* x, int x_ld, void* y, int y_ld, int
                                  y5_stream_t stream) {
     return y5_launch_upsample2x(x, x_ld, y, y_ld, batch, h, w, c, mode, static_cast<hipStream_t>(stream));
 }
+extern "C" int y5_group_norm_workspace(const y5_group_norm_desc* d, int what, size_t* bytes) {
+    Y5_REQUIRE(d && bytes, "group_norm_workspace: null argument");
+    return y5_group_norm_work(*d, what, bytes);
+}
+extern "C" int y5_group_norm(const y5_group_norm_desc* d, y5_stream_t stream) {
+    Y5_REQUIRE(d, "group_norm: null descriptor");
+    return y5_launch_group_norm(*d, static_cast<hipStream_t>(stream));
+}
+extern "C" int y5_group_norm_backward(const y5_group_norm_desc* d, y5_stream_t stream) {
+    Y5_REQUIRE(d, "group_norm_backward: null descriptor");
+    return y5_launch_group_norm_bwd(*d, static_cast<hipStream_t>(stream));
+}
+extern "C" int y5_group_norm_rows_i8(const y5_group_norm_desc* d, void* q, int q_ld, float* scale, y5_stream_t stream) {
+    Y5_REQUIRE(d, "group_norm_rows: null descriptor");
+    return y5_launch_group_norm_rows(*d, q, q_ld, scale, static_cast<hipStream_t>(stream));
+}
+extern "C" int y5_quantize_rows_i8(const void* x, int64_t x_ld, int dtype, int64_t rows, int k, void* q, int q_ld, float* scale, y5_stream_t stream) {
+    return y5_launch_quantize_rows(x, x_ld, dtype, rows, k, q, q_ld, scale, static_cast<hipStream_t>(stream));
+}
+extern "C" int y5_gemm_i8(const y5_gemm_i8_desc* d, y5_stream_t stream) {
+    Y5_REQUIRE(d, "gemm_i8: null descriptor");
+    return y5_launch_gemm_i8(*d, static_cast<hipStream_t>(stream));
+}
+
 extern "C" int y5_conv_stats_f16(const y5_conv_desc* d, float* partials, int rows, int stats_c, int stats_off, y5_stream_t stream) {
     Y5_REQUIRE(d, "conv_stats: null descriptor");
     const Y5ConvStats st{partials, rows, stats_c, stats_off};

@@ -1,0 +1,316 @@
+// Rows of 8-bit integers with a scale a row, from 16- or 32-bit values (y5_quantize_rows_i8) or straight from a group norm
+// with its activation (y5_group_norm_rows_i8): a = max |v| of the row, scale = a / 127, q = the whole number nearest to
+// 127 v / a.  Rows with a below 2^-120 (127 / a would overflow) count as zero: scale 0.  A row with an infinity or a NaN gets
+// the scale NaN and zeros, so that everything computed from it is NaN.
+//
+// Memory bound: a value is read once, and written as one byte.  A row lives in the registers of the lanes that read it, so the
+// maximum is a few shuffles; with the group norm the normalised value is rounded once, to 8 bits, and no 16-bit tensor in between
+// is written or read.
+#include "y5_common.h"
+
+namespace {
+
+#include "norm_rows.h"
+
+constexpr float kZeroRow = 7.52316384526264e-37f;  // 2^-120
+
+struct RowsArgs {
+    const void* x;
+    signed char* q;
+    float* scale;
+    long long rows, x_ld;
+    int k, q_ld;   // values of a row; bytes of a row of q (a multiple of 16; zeros behind the k-th)
+    int lanes;     // lanes of a row (a power of two up to 64)
+    int run;       // rows of a workgroup
+    // with the group norm only
+    NormShape s;
+    const float2* part;
+    const void *weight, *bias;
+};
+
+// The multiplier of a row with the largest magnitude `bits` (as the bits of a float); 0 for a row of zeros.
+__device__ __forceinline__ float row_scale(unsigned bits, float* a) {
+    const float m = __uint_as_float(bits);
+    *a = m >= kZeroRow ? m : 0.f;
+    if (bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+    return *a / 127.f;
+}
+
+// The whole number nearest to v * 127 / a.  fp32 values are scaled in 64 bits: their 24 digits leave no room for an error of
+// the multiplication, which would put values next to a half on its other side.  16-bit values have 13 digits of room.
+struct Inv32 {
+    float f;
+    __device__ __forceinline__ void set(float a, bool ok) { f = ok && a > 0.f ? 127.f / a : 0.f; }
+    __device__ __forceinline__ int operator()(float v) const { return (int)__builtin_rintf(v * f); }
+};
+struct Inv64 {
+    double f;
+    __device__ __forceinline__ void set(float a, bool ok) { f = ok && a > 0.f ? 127.0 / (double)a : 0.0; }
+    __device__ __forceinline__ int operator()(float v) const { return (int)__builtin_rint((double)v * f); }
+};
+template <typename T, bool NORM>
+struct InvOf {
+    typedef Inv32 type;
+};
+template <>
+struct InvOf<float, false> {
+    typedef Inv64 type;
+};
+
+// V bytes of a row
+template <int V>
+__device__ __forceinline__ void st_bytes(signed char* p, const int (&v)[V]) {
+    unsigned w[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i)
+        w[i] = (unsigned)(v[4 * i] & 255) | (unsigned)(v[4 * i + 1] & 255) << 8 | (unsigned)(v[4 * i + 2] & 255) << 16 | (unsigned)v[4 * i + 3] << 24;
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<unsigned*>(p) = w[0];
+}
+
+// Lanes share a row: vector v of lane l covers elements ((v * lanes) + l) * V.  NV vectors a lane.
+// grid: runs of `run` rows (x batch with NORM, where a workgroup's rows are pixels of one image)
+// LDS with NORM: red[2 * blockDim.x], gmean, grstd[groups], A[q_ld], B[q_ld] (z = x * A + B)
+template <typename T, bool NORM, int NV>
+__global__ __launch_bounds__(256) void rows_kernel(const RowsArgs a) {
+    constexpr int V = NormElem<T>::V;
+    extern __shared__ float lds[];
+    const int t = threadIdx.x, TB = blockDim.x;
+    const int l = t & (a.lanes - 1);
+    long long row0 = (long long)blockIdx.x * a.run, rows = a.rows, base = 0;
+    float* coef = nullptr;
+    if constexpr (NORM) {
+        const NormShape& s = a.s;
+        const int b = s.batch - 1 - blockIdx.y;  // from the end: the statistics pass read that last
+        row0 = (long long)(gridDim.x - 1 - blockIdx.x) * a.run;
+        rows = s.pixels;
+        base = (long long)b * s.pixels;
+        float *red = lds, *gmean = red + 2 * TB, *grstd = gmean + s.groups;
+        coef = grstd + s.groups;
+        norm_merge_chunks(s, a.part, b, red, gmean, grstd);
+        // mean and beta in one number: what that costs (the mean's magnitude over a deviation, times 2^-24) is far below the
+        // 2^-8 of the rounding that follows
+        for (int c = t; c < a.q_ld; c += TB) {
+            float A = 0.f, B = 0.f;
+            if (c < s.c) {
+                const int g = c / s.cpg;
+                A = ld_param(a.weight, c, s.param_dtype, 1.f) * grstd[g];
+                B = __builtin_fmaf(-gmean[g], A, ld_param(a.bias, c, s.param_dtype, 0.f));
+            }
+            coef[c] = A;
+            coef[a.q_ld + c] = B;
+        }
+        __syncthreads();
+    }
+    int off[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) off[v] = (v * a.lanes + l) * V;
+    const long long row1 = row0 + a.run < rows ? row0 + a.run : rows;
+    const int step = TB / a.lanes;
+    // every lane of a wave takes every turn: a row of lanes past the end reads and writes nothing
+    for (long long first = row0; first < row1; first += step) {
+        const long long row = first + t / a.lanes;
+        const bool on = row < row1;
+        const T* xr = static_cast<const T*>(a.x) + (base + row) * a.x_ld;
+        T x[NV][V];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int n = on ? a.k - off[v] : 0;
+            if (n >= V) ld_vec(xr + off[v], x[v]);
+            else ld_part(xr + off[v], n, x[v]);
+        }
+        unsigned top = 0;
+        float z[NORM ? NV : 1][V];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            float f[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = (float)x[v][e];
+            if constexpr (NORM) {
+                if (off[v] < a.q_ld) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) f[e] = __builtin_fmaf(f[e], coef[off[v] + e], coef[a.q_ld + off[v] + e]);
+                    norm_act(f, a.s.act, a.s.slope);
+                }
+#pragma unroll
+                for (int e = 0; e < V; ++e) z[v][e] = f[e];
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const unsigned u = __float_as_uint(f[e]) & 0x7fffffffu;  // NaN > infinity > every number
+                top = u > top ? u : top;
+            }
+        }
+        for (int d = a.lanes >> 1; d; d >>= 1) {
+            const unsigned u = (unsigned)__shfl_xor((int)top, d);
+            top = u > top ? u : top;
+        }
+        float m;
+        const float scale = row_scale(top, &m);
+        typename InvOf<T, NORM>::type inv;
+        inv.set(m, top < 0x7f800000u);
+        if (!on) continue;
+        signed char* qr = a.q + (size_t)(base + row) * a.q_ld;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if (off[v] >= a.q_ld) continue;
+            int w[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) w[e] = top < 0x7f800000u ? inv(NORM ? z[NORM ? v : 0][e] : (float)x[v][e]) : 0;
+            st_bytes<V>(qr + off[v], w);
+        }
+        if (l == 0) a.scale[base + row] = scale;
+    }
+}
+
+// One workgroup a row: long rows, or few of them.  The row is read twice, the second time from the cache.
+template <typename T>
+__global__ __launch_bounds__(256) void long_rows_kernel(const RowsArgs a) {
+    constexpr int V = NormElem<T>::V;
+    __shared__ unsigned tops[4];
+    const int t = threadIdx.x;
+    const long long row = blockIdx.x;
+    const T* xr = static_cast<const T*>(a.x) + row * a.x_ld;
+    unsigned top = 0;
+    for (int off = t * V; off < a.k; off += 256 * V) {
+        T x[V];
+        if (a.k - off >= V) ld_vec(xr + off, x);
+        else ld_part(xr + off, a.k - off, x);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const unsigned u = __float_as_uint((float)x[e]) & 0x7fffffffu;
+            top = u > top ? u : top;
+        }
+    }
+    for (int d = 32; d; d >>= 1) {
+        const unsigned u = (unsigned)__shfl_xor((int)top, d);
+        top = u > top ? u : top;
+    }
+    if ((t & 63) == 0) tops[t >> 6] = top;
+    __syncthreads();
+    top = tops[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) top = tops[i] > top ? tops[i] : top;
+    float m;
+    const float scale = row_scale(top, &m);
+    typename InvOf<T, false>::type inv;
+    inv.set(m, top < 0x7f800000u);
+    for (int off = t * V; off < a.q_ld; off += 256 * V) {
+        T x[V];
+        if (a.k - off >= V) ld_vec(xr + off, x);
+        else ld_part(xr + off, a.k - off, x);
+        int w[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[e] = top < 0x7f800000u ? inv((float)x[e]) : 0;
+        st_bytes<V>(a.q + (size_t)row * a.q_ld + off, w);
+    }
+    if (t == 0) a.scale[row] = scale;
+}
+
+template <typename T>
+int quantize(RowsArgs a, hipStream_t st) {
+    constexpr int V = NormElem<T>::V;
+    const int vecs = a.q_ld / V;
+    if (vecs > 64 * 8) {  // more than a wave's registers hold
+        hipLaunchKernelGGL((long_rows_kernel<T>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
+        Y5_LAUNCH_CHECK("long_rows_kernel");
+        return Y5_OK;
+    }
+    a.lanes = 1;
+    while (a.lanes < 64 && a.lanes < vecs) a.lanes *= 2;
+    const int nv = (vecs + a.lanes - 1) / a.lanes;
+    const int step = 256 / a.lanes;  // rows of a workgroup in one turn
+    // four turns a workgroup, fewer where that would leave the chip empty
+    int turns = 4;
+    while (turns > 1 && a.rows / ((long long)step * turns) < 1024) turns /= 2;
+    a.run = step * turns;
+    const dim3 grid((unsigned)((a.rows + a.run - 1) / a.run));
+    if (nv == 1) hipLaunchKernelGGL((rows_kernel<T, false, 1>), grid, dim3(256), 0, st, a);
+    else if (nv == 2) hipLaunchKernelGGL((rows_kernel<T, false, 2>), grid, dim3(256), 0, st, a);
+    else if (nv <= 4) hipLaunchKernelGGL((rows_kernel<T, false, 4>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((rows_kernel<T, false, 8>), grid, dim3(256), 0, st, a);
+    Y5_LAUNCH_CHECK("rows_kernel");
+    return Y5_OK;
+}
+
+template <typename T>
+int norm_rows(RowsArgs a, hipStream_t st) {
+    constexpr int V = NormElem<T>::V;
+    const int vecs = a.q_ld / V;
+    a.lanes = 1;
+    while (a.lanes < 64 && a.lanes < vecs) a.lanes *= 2;
+    const int nv = (vecs + a.lanes - 1) / a.lanes;
+    const int step = 256 / a.lanes;
+    // rows of a workgroup: 32 KiB of them, so that merging the statistics is little beside it
+    long long run = (32 << 10) / ((long long)a.k * (int)sizeof(T));
+    run = run < step ? step : run / step * step;
+    a.run = (int)run;
+    const dim3 grid((unsigned)((a.s.pixels + run - 1) / run), (unsigned)a.s.batch);
+    const size_t lds = (2 * 256 + 2 * (size_t)a.s.groups + 2 * (size_t)a.q_ld) * 4;  // at most 2 + 32 + 32 KiB + 128
+    auto launch = [&](auto kernel) -> int {
+        if (lds > 64 << 10) Y5_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, a);
+        Y5_LAUNCH_CHECK("rows_kernel");
+        return Y5_OK;
+    };
+    if (nv == 1) return launch(rows_kernel<T, true, 1>);
+    if (nv == 2) return launch(rows_kernel<T, true, 2>);
+    if (nv <= 4) return launch(rows_kernel<T, true, 4>);
+    if constexpr (V == 4) {
+        if (nv > 8) return launch(rows_kernel<T, true, 16>);
+    }
+    return launch(rows_kernel<T, true, 8>);
+}
+
+int check_rows(const char* name, const void* q, const void* scale, int k, int q_ld) {
+    Y5_REQUIRE(q && scale, "%s: null output", name);
+    Y5_REQUIRE(k > 0 && k <= Y5_I8_MAX_K, "%s: %d values a row (1 to %d)", name, k, Y5_I8_MAX_K);
+    Y5_REQUIRE(q_ld == (k + 15) / 16 * 16, "%s: a row of q is %d bytes for %d values (got %d)", name, (k + 15) / 16 * 16, k, q_ld);
+    Y5_REQUIRE(y5_aligned16(q) && reinterpret_cast<uintptr_t>(scale) % 4 == 0, "%s: misaligned output", name);
+    return Y5_OK;
+}
+
+}  // namespace
+
+int y5_launch_quantize_rows(const void* x, int64_t x_ld, int dtype, int64_t rows, int k, void* q, int q_ld, float* scale, hipStream_t st) {
+    Y5_REQUIRE(x, "quantize_rows: null x");
+    Y5_REQUIRE(dtype == Y5_F16 || dtype == Y5_BF16 || dtype == Y5_F32, "quantize_rows: dtype %d", dtype);
+    if (int rc = check_rows("quantize_rows", q, scale, k, q_ld)) return rc;
+    Y5_REQUIRE(rows > 0 && rows <= 0x7fffffff, "quantize_rows: %lld rows", (long long)rows);
+    Y5_REQUIRE(x_ld >= k, "quantize_rows: pitch %lld for %d values", (long long)x_ld, k);
+    Y5_REQUIRE(reinterpret_cast<uintptr_t>(x) % norm_elem_size(dtype) == 0, "quantize_rows: misaligned x");
+    RowsArgs a{};
+    a.x = x;
+    a.q = static_cast<signed char*>(q);
+    a.scale = scale;
+    a.rows = rows;
+    a.x_ld = x_ld;
+    a.k = k;
+    a.q_ld = q_ld;
+    if (dtype == Y5_F16) return quantize<f16>(a, st);
+    if (dtype == Y5_BF16) return quantize<bf16>(a, st);
+    return quantize<float>(a, st);
+}
+
+int y5_launch_group_norm_rows(const y5_group_norm_desc& d, void* q, int q_ld, float* scale, hipStream_t st) {
+    RowsArgs a{};
+    if (int rc = norm_make_shape(d, &a.s)) return rc;
+    if (int rc = norm_check_pitch(d, a.s, "x", d.x, d.x_ld)) return rc;
+    if (int rc = check_rows("group_norm_rows", q, scale, d.c, q_ld)) return rc;
+    const size_t need = (size_t)a.s.batch * a.s.chunks * a.s.groups * sizeof(float2);
+    if (!d.workspace || d.workspace_bytes < need) return y5_fail(Y5_EWORKSPACE, "group_norm_rows: workspace of %zu bytes, %zu needed", d.workspace ? d.workspace_bytes : (size_t)0, need);
+    Y5_REQUIRE(y5_aligned16(d.workspace), "group_norm_rows: misaligned workspace");
+    if (int rc = y5_launch_group_norm_stats(d, st)) return rc;
+    a.x = d.x;
+    a.q = static_cast<signed char*>(q);
+    a.scale = scale;
+    a.x_ld = d.x_ld;
+    a.k = d.c;
+    a.q_ld = q_ld;
+    a.part = static_cast<const float2*>(d.workspace);
+    a.weight = d.weight;
+    a.bias = d.bias;
+    if (d.dtype == Y5_F16) return norm_rows<f16>(a, st);
+    if (d.dtype == Y5_BF16) return norm_rows<bf16>(a, st);
+    return norm_rows<float>(a, st);
+}

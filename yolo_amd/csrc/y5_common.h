@@ -171,3 +171,12 @@ int y5_launch_bn_finalize(const float* partials, int rows, long long count, int 
                           hipStream_t s);
 int y5_launch_affine_act(const void* x, int x_ld, void* y, int y_ld, const void* res, int res_ld, long long pixels, int c,
                          const float* scale, const float* shift, int act, float slope, hipStream_t s);
+// Group norm, channels last (groupnorm.hip); the statistics pass alone leaves the chunks' statistics in d.workspace
+int y5_group_norm_work(const y5_group_norm_desc& d, int what, size_t* bytes);
+int y5_launch_group_norm(const y5_group_norm_desc& d, hipStream_t s);
+int y5_launch_group_norm_bwd(const y5_group_norm_desc& d, hipStream_t s);
+int y5_launch_group_norm_stats(const y5_group_norm_desc& d, hipStream_t s);
+// 8-bit rows (rows_i8.hip) and their product (gemm_i8.hip)
+int y5_launch_quantize_rows(const void* x, int64_t x_ld, int dtype, int64_t rows, int k, void* q, int q_ld, float* scale, hipStream_t s);
+int y5_launch_group_norm_rows(const y5_group_norm_desc& d, void* q, int q_ld, float* scale, hipStream_t s);
+int y5_launch_gemm_i8(const y5_gemm_i8_desc& d, hipStream_t s);
