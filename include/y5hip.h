@@ -485,6 +485,12 @@ typedef struct y5_gemm_i8_desc {
     float slope;
 } y5_gemm_i8_desc;
 int y5_gemm_i8(const y5_gemm_i8_desc* d, y5_stream_t stream);
+/* y5_quantize_rows_i8 and y5_gemm_i8 as one call: x are d->m rows of d->k values of x_dtype at pitch x_ld (d->a and d->a_scale are
+ * not used).  The same bits as the two calls; where the shape allows, the rows are quantised inside the product.
+ * workspace: y5_linear_i8_workspace bytes (may be 0), 16-byte aligned, used until the call's work on the stream is done. */
+int y5_linear_i8_workspace(const y5_gemm_i8_desc* d, int x_dtype, size_t* bytes);
+int y5_linear_i8(const y5_gemm_i8_desc* d, const void* x, int64_t x_ld, int x_dtype, void* workspace, size_t workspace_bytes,
+                 y5_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * Launch plans: a host-side list of the calls above, replayed with one C call per forward.

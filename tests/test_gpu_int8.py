@@ -66,7 +66,8 @@ def test_quantize_rows_extremes(dev):
 
 
 def product_ref(q, scale, w, wscale, bias, act, slope):
-    s = (q.cpu().double() @ w.cpu().double().t()) * (scale.cpu().double()[:, None] * wscale.cpu().double())
+    whole = q.double() @ w.double().t()  # exact
+    s = whole.cpu() * (scale.cpu().double()[:, None] * wscale.cpu().double())
     b = torch.zeros(w.shape[0]).double() if bias is None else bias.cpu().double()
     z = s + b
     return act_ref(z, act, slope), 4 * E32 * (s.abs() + b.abs()) + (8 * E32 * z.abs() if act == 'silu' else 0)
@@ -75,7 +76,8 @@ def product_ref(q, scale, w, wscale, bias, act, slope):
 # rows x values x channels: one of each; every edge of a 16-value vector, a 64-value fragment and a tile; the head's 255 channels; rows of
 # one token up to several tiles; long rows with few channels and the reverse
 PRODUCTS = [(1, 1, 1), (1, 16, 16), (2, 17, 3), (1, 4096, 512), (3, 1000, 255), (16, 64, 64), (17, 65, 33), (64, 128, 128), (65, 129, 257), (333, 1000, 255),
-            (300, 80, 72), (1000, 32, 64), (515, 256, 256), (129, 2048, 130), (8, 20000, 24), (4, 640, 4100), (2049, 63, 40), (1030, 520, 392), (700, 1280, 700)]
+            (300, 80, 72), (1000, 32, 64), (515, 256, 256), (129, 2048, 130), (8, 20000, 24), (4, 640, 4100), (2049, 63, 40), (1030, 520, 392), (700, 1280, 700),
+            (20, 2048, 2064), (4100, 60, 130), (66000, 128, 72), (2000, 500, 2040), (4090, 512, 2048), (16300, 2000, 1000)]
 
 
 @pytest.mark.parametrize('dtype', [F16, BF16, F32], ids=['fp16', 'bf16', 'fp32'])
@@ -90,7 +92,7 @@ def test_product(dev, m, k, n, dtype):
         w[0] = -128
     s, ws = torch.rand(m, generator=g) * 0.02 + 1e-3, (torch.rand(n, generator=g) + 0.1) * 0.02 / k ** 0.5
     bias = None if n % 2 else torch.randn(n, generator=g)
-    want, err = product_ref(q, s, w, ws, bias, act, 0.2)
+    want, err = product_ref(q.to(dev), s, w.to(dev), ws, bias, act, 0.2)
     rows = Int8Rows(torch.nn.functional.pad(q, (0, row_bytes(k) - k)).to(dev), s.to(dev), (m,), k, dtype)
     y = linear_i8(rows, Int8Weight(w.to(dev), ws.to(dev)), None if bias is None else bias.to(dev), act=act, slope=0.2)
     assert y.dtype is dtype
@@ -98,7 +100,8 @@ def test_product(dev, m, k, n, dtype):
 
 
 @pytest.mark.parametrize('dtype', [F16, BF16, F32], ids=['fp16', 'bf16', 'fp32'])
-@pytest.mark.parametrize('m,k,n', [(1, 4096, 96), (2, 30, 7), (5, 257, 300), (13, 1024, 64), (16, 640, 255), (31, 96, 17), (77, 200, 64), (900, 64, 64), (1111, 72, 24), (513, 512, 130), (640, 250, 256)])
+@pytest.mark.parametrize('m,k,n', [(1, 4096, 96), (2, 30, 7), (5, 257, 300), (13, 1024, 64), (16, 640, 255), (31, 96, 17), (77, 200, 64), (900, 64, 64), (1111, 72, 24), (513, 512, 130), (640, 250, 256),
+                                   (2100, 48, 130), (17000, 128, 80), (16500, 240, 33), (16400, 512, 64), (16400, 256, 528), (16400, 272, 20), (4, 16384, 24), (3, 21848, 40)])
 def test_linear_from_floating_point(dev, m, k, n, dtype):
     """linear_i8 of a tensor is the product of its quantised rows: the same bits as in two calls, and those within tolerance."""
     g = torch.Generator().manual_seed(m * 7 + k + n)

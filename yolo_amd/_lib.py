@@ -116,6 +116,8 @@ SIGNATURES = {
     'y5_group_norm_rows_i8': (_i, [C.POINTER(GroupNormDesc), _p, _i, _p, _s]),
     'y5_quantize_rows_i8': (_i, [_p, C.c_int64, _i, C.c_int64, _i, _p, _i, _p, _s]),
     'y5_gemm_i8': (_i, [C.POINTER(GemmI8Desc), _s]),
+    'y5_linear_i8_workspace': (_i, [C.POINTER(GemmI8Desc), _i, C.POINTER(C.c_size_t)]),
+    'y5_linear_i8': (_i, [C.POINTER(GemmI8Desc), _p, C.c_int64, _i, _p, C.c_size_t, _s]),
     'y5_detect_decode_f16': (_i, [C.POINTER(DecodeDesc), _s]),
     'y5_detect_decode_multi_f16': (_i, [C.POINTER(DecodeDesc), C.c_int, _s]),
     'y5_detect_f16': (_i, [C.POINTER(ConvDesc), C.POINTER(DecodeDesc), C.c_int, _s]),

@@ -125,6 +125,14 @@ extern "C" int y5_group_norm_rows_i8(const y5_group_norm_desc* d, void* q, int q
 extern "C" int y5_quantize_rows_i8(const void* x, int64_t x_ld, int dtype, int64_t rows, int k, void* q, int q_ld, float* scale, y5_stream_t stream) {
     return y5_launch_quantize_rows(x, x_ld, dtype, rows, k, q, q_ld, scale, static_cast<hipStream_t>(stream));
 }
+extern "C" int y5_linear_i8_workspace(const y5_gemm_i8_desc* d, int x_dtype, size_t* bytes) {
+    Y5_REQUIRE(d && bytes, "linear_i8_workspace: null argument");
+    return y5_linear_i8_work(*d, x_dtype, bytes);
+}
+extern "C" int y5_linear_i8(const y5_gemm_i8_desc* d, const void* x, int64_t x_ld, int x_dtype, void* workspace, size_t workspace_bytes, y5_stream_t stream) {
+    Y5_REQUIRE(d, "linear_i8: null descriptor");
+    return y5_launch_linear_i8(*d, x, x_ld, x_dtype, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
 extern "C" int y5_gemm_i8(const y5_gemm_i8_desc* d, y5_stream_t stream) {
     Y5_REQUIRE(d, "gemm_i8: null descriptor");
     return y5_launch_gemm_i8(*d, static_cast<hipStream_t>(stream));

@@ -9,15 +9,21 @@ struct NormElem {
 };
 
 // A pixel of a tensor whose channel count or pitch is not a multiple of 8 starts anywhere: the accesses below are 16 bytes at
-// element alignment, which the memory pipeline serves like aligned ones, in one or two more cache lines.
+// element alignment, which the memory pipeline serves like aligned ones, in one or two more cache lines.  One 16-byte value, not
+// V elements: as elements the compiler splits such an access up where a branch beside it touches some of them.
+typedef unsigned norm_u32x4 __attribute__((ext_vector_type(4)));
 template <typename T>
 struct __attribute__((packed, aligned(sizeof(T)))) NormVec {
+    norm_u32x4 v;
+};
+template <typename T>
+struct NormArr {
     T v[NormElem<T>::V];
 };
 
 template <typename T>
 __device__ __forceinline__ void ld_vec(const T* p, T (&v)[NormElem<T>::V]) {
-    const NormVec<T> u = *reinterpret_cast<const NormVec<T>*>(p);
+    const NormArr<T> u = __builtin_bit_cast(NormArr<T>, reinterpret_cast<const NormVec<T>*>(p)->v);
 #pragma unroll
     for (int e = 0; e < NormElem<T>::V; ++e) v[e] = u.v[e];
 }
@@ -32,10 +38,10 @@ __device__ __forceinline__ void ld_part(const T* p, int n, T (&v)[NormElem<T>::V
 }
 template <typename T>
 __device__ __forceinline__ void st_vec(T* p, const T (&v)[NormElem<T>::V]) {
-    NormVec<T> u;
+    NormArr<T> u;
 #pragma unroll
     for (int e = 0; e < NormElem<T>::V; ++e) u.v[e] = v[e];
-    *reinterpret_cast<NormVec<T>*>(p) = u;
+    reinterpret_cast<NormVec<T>*>(p)->v = __builtin_bit_cast(norm_u32x4, u);
 }
 template <typename T>
 __device__ __forceinline__ void st_part(T* p, int n, const T (&v)[NormElem<T>::V]) {

@@ -11,8 +11,7 @@
 namespace {
 
 #include "norm_rows.h"
-
-constexpr float kZeroRow = 7.52316384526264e-37f;  // 2^-120
+#include "quant_rows.h"
 
 struct RowsArgs {
     const void* x;
@@ -28,44 +27,11 @@ struct RowsArgs {
     const void *weight, *bias;
 };
 
-// The multiplier of a row with the largest magnitude `bits` (as the bits of a float); 0 for a row of zeros.
-__device__ __forceinline__ float row_scale(unsigned bits, float* a) {
-    const float m = __uint_as_float(bits);
-    *a = m >= kZeroRow ? m : 0.f;
-    if (bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
-    return *a / 127.f;
-}
-
-// The whole number nearest to v * 127 / a.  fp32 values are scaled in 64 bits: their 24 digits leave no room for an error of
-// the multiplication, which would put values next to a half on its other side.  16-bit values have 13 digits of room.
-struct Inv32 {
-    float f;
-    __device__ __forceinline__ void set(float a, bool ok) { f = ok && a > 0.f ? 127.f / a : 0.f; }
-    __device__ __forceinline__ int operator()(float v) const { return (int)__builtin_rintf(v * f); }
-};
-struct Inv64 {
-    double f;
-    __device__ __forceinline__ void set(float a, bool ok) { f = ok && a > 0.f ? 127.0 / (double)a : 0.0; }
-    __device__ __forceinline__ int operator()(float v) const { return (int)__builtin_rint((double)v * f); }
-};
-template <typename T, bool NORM>
-struct InvOf {
-    typedef Inv32 type;
-};
-template <>
-struct InvOf<float, false> {
-    typedef Inv64 type;
-};
-
 // V bytes of a row
 template <int V>
 __device__ __forceinline__ void st_bytes(signed char* p, const int (&v)[V]) {
-    unsigned w[V / 4];
-#pragma unroll
-    for (int i = 0; i < V / 4; ++i)
-        w[i] = (unsigned)(v[4 * i] & 255) | (unsigned)(v[4 * i + 1] & 255) << 8 | (unsigned)(v[4 * i + 2] & 255) << 16 | (unsigned)v[4 * i + 3] << 24;
-    if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-    else *reinterpret_cast<unsigned*>(p) = w[0];
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(pack_bytes(v[0], v[1], v[2], v[3]), pack_bytes(v[4], v[5], v[6], v[7]));
+    else *reinterpret_cast<int*>(p) = pack_bytes(v[0], v[1], v[2], v[3]);
 }
 
 // Lanes share a row: vector v of lane l covers elements ((v * lanes) + l) * V.  NV vectors a lane.
@@ -136,10 +102,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsArgs a) {
                 for (int e = 0; e < V; ++e) z[v][e] = f[e];
             }
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const unsigned u = __float_as_uint(f[e]) & 0x7fffffffu;  // NaN > infinity > every number
-                top = u > top ? u : top;
-            }
+            for (int e = 0; e < V; ++e) top = max_bits(top, f[e]);
         }
         for (int d = a.lanes >> 1; d; d >>= 1) {
             const unsigned u = (unsigned)__shfl_xor((int)top, d);
@@ -177,10 +140,7 @@ __global__ __launch_bounds__(256) void long_rows_kernel(const RowsArgs a) {
         if (a.k - off >= V) ld_vec(xr + off, x);
         else ld_part(xr + off, a.k - off, x);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const unsigned u = __float_as_uint((float)x[e]) & 0x7fffffffu;
-            top = u > top ? u : top;
-        }
+        for (int e = 0; e < V; ++e) top = max_bits(top, (float)x[e]);
     }
     for (int d = 32; d; d >>= 1) {
         const unsigned u = (unsigned)__shfl_xor((int)top, d);

@@ -180,3 +180,12 @@ int y5_launch_group_norm_stats(const y5_group_norm_desc& d, hipStream_t s);
 int y5_launch_quantize_rows(const void* x, int64_t x_ld, int dtype, int64_t rows, int k, void* q, int q_ld, float* scale, hipStream_t s);
 int y5_launch_group_norm_rows(const y5_group_norm_desc& d, void* q, int q_ld, float* scale, hipStream_t s);
 int y5_launch_gemm_i8(const y5_gemm_i8_desc& d, hipStream_t s);
+int y5_linear_i8_work(const y5_gemm_i8_desc& d, int x_dtype, size_t* bytes);
+int y5_launch_linear_i8(const y5_gemm_i8_desc& d, const void* x, int64_t x_ld, int x_dtype, void* workspace, size_t workspace_bytes, hipStream_t s);
+// many rows of few values (gemm_i8_rows.hip): whether the shape is covered; x: rows of d.dtype to quantise, or nullptr for d.a
+bool y5_gemm_rows_fits(int n, int k, bool quantise, int dtype);
+int y5_launch_gemm_rows(const y5_gemm_i8_desc& d, const void* x, int64_t x_ld, hipStream_t s);
+// few rows, or few outputs of few values (gemm_i8_few.hip); x: up to Y5_FEW_ROWS rows of d.dtype to quantise, or nullptr for d.a;
+// rows: 16 or 32 a workgroup (16 with x)
+#define Y5_FEW_ROWS 4
+int y5_launch_gemm_few(const y5_gemm_i8_desc& d, const void* x, int64_t x_ld, int rows, hipStream_t s);

@@ -19,7 +19,7 @@ import torch
 import torch.nn as nn
 
 from yolo_amd import _lib
-from yolo_amd.groupnorm import _ACTS, _DTYPES, act_code, apply_act, channels_last, on_device, pixel_pitch
+from yolo_amd.groupnorm import _ACTS, _DTYPES, act_code, apply_act, on_device, pixel_pitch
 
 ZERO_ROW = 2.0 ** -120
 
@@ -120,6 +120,16 @@ def _quantize(x, pitch, lead, k):
     return rows
 
 
+def _rows_of(x):
+    """x (..., k) as rows at one pitch: itself where its memory is that, else a copy."""
+    k = x.shape[-1]
+    if x.dim() != 2 or x.stride(1) != 1 or x.stride(0) < k:
+        x = x.reshape(-1, k)
+        if (k > 1 and x.stride(1) != 1) or x.stride(0) < k:
+            x = x.contiguous()
+    return x, max(x.stride(0), k)
+
+
 def quantize_rows(x):
     """x (..., k), fp16 / bf16 / fp32 -> Int8Rows with a scale a row of the last dimension."""
     if x.dtype not in _DTYPES:
@@ -131,11 +141,8 @@ def quantize_rows(x):
     _check_k(k)
     if not x.is_cuda or x.numel() == 0:
         return _quantize_plain(x, lead, k, x.dtype)
-    if x.dim() != 2 or x.stride(1) != 1 or x.stride(0) < k:
-        x = x.reshape(-1, k)
-        if (x.shape[1] > 1 and x.stride(1) != 1) or x.stride(0) < k:
-            x = x.contiguous()
-    return _quantize(x, max(x.stride(0), k), lead, k)
+    x, pitch = _rows_of(x)
+    return _quantize(x, pitch, lead, k)
 
 
 def quantize_weight(w):
@@ -148,20 +155,41 @@ def quantize_weight(w):
     return Int8Weight(rows.q[:, :rows.k], rows.scale)
 
 
+def _plain_product(rows, weight, bias, act, slope, dtype):
+    y = rows.q[:, :rows.k].double() @ weight.q[:, :weight.k].double().t()
+    y = y.float() * (rows.scale[:, None] * weight.scale)
+    y = y if bias is None else y + bias
+    return apply_act(y, act, slope).to(dtype)
+
+
+def _desc(rows, weight, bias, act, slope, y, m):
+    return _lib.GemmI8Desc(None if rows is None else rows.q.data_ptr(), None if rows is None else rows.scale.data_ptr(), weight.q.data_ptr(),
+                           weight.scale.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), m, weight.n, weight.n, weight.k,
+                           weight.q.shape[1], _DTYPES[y.dtype], _ACTS[act], slope)
+
+
 def _product(rows, weight, bias, act, slope, dtype):
-    """(rows, n) of dtype."""
+    """(rows, n) of dtype from Int8Rows."""
     m = rows.q.shape[0]
     if not rows.q.is_cuda or m == 0:
-        y = rows.q[:, :rows.k].double() @ weight.q[:, :weight.k].double().t()
-        y = y.float() * (rows.scale[:, None] * weight.scale)
-        y = y if bias is None else y + bias
-        return apply_act(y, act, slope).to(dtype)
+        return _plain_product(rows, weight, bias, act, slope, dtype)
     with on_device(rows.q):
         y = torch.empty((m, weight.n), dtype=dtype, device=rows.q.device)
-        d = _lib.GemmI8Desc(rows.q.data_ptr(), rows.scale.data_ptr(), weight.q.data_ptr(), weight.scale.data_ptr(),
-                            None if bias is None else bias.data_ptr(), y.data_ptr(), m, weight.n, weight.n, weight.k, rows.q.shape[1],
-                            _DTYPES[dtype], _ACTS[act], slope)
-        _lib.check(_lib.lib().y5_gemm_i8(C.byref(d), _lib.current_stream()))
+        _lib.check(_lib.lib().y5_gemm_i8(C.byref(_desc(rows, weight, bias, act, slope, y, m)), _lib.current_stream()))
+    return y
+
+
+def _linear(x, pitch, m, weight, bias, act, slope, dtype):
+    """(m, n) of dtype from m rows `pitch` elements apart, quantised on the way."""
+    with on_device(x):
+        lib = _lib.lib()
+        y = torch.empty((m, weight.n), dtype=dtype, device=x.device)
+        d = _desc(None, weight, bias, act, slope, y, m)
+        n = C.c_size_t()
+        _lib.check(lib.y5_linear_i8_workspace(C.byref(d), _DTYPES[x.dtype], C.byref(n)))
+        ws = torch.empty(n.value, dtype=torch.uint8, device=x.device) if n.value else None
+        _lib.check(lib.y5_linear_i8(C.byref(d), x.data_ptr(), pitch, _DTYPES[x.dtype], None if ws is None else ws.data_ptr(), n.value,
+                                    _lib.current_stream()))
     return y
 
 
@@ -188,13 +216,20 @@ def linear_i8(x, weight, bias=None, act=None, slope=0.1, dtype=None):
     weight: Int8Weight; bias: (n) or None; act: None, 'leaky' (with slope) or 'silu'.  The result is (..., n) of type dtype
     (x's own by default)."""
     rows = isinstance(x, Int8Rows)
-    bias = _check('linear_i8', x, weight, bias, act, dtype or x.dtype)
+    dtype = dtype or x.dtype
+    bias = _check('linear_i8', x, weight, bias, act, dtype)
     k = x.k if rows else x.shape[-1] if x.dim() else 0
     if k != weight.k:
         raise ValueError('rows of %d values, weights for %d' % (k, weight.k))
-    lead = x.lead if rows else x.shape[:-1]
-    y = _product(x if rows else quantize_rows(x), weight, bias, act, slope, dtype or x.dtype)
-    return y.reshape(*lead, weight.n)
+    if rows:
+        return _product(x, weight, bias, act, slope, dtype).reshape(*x.lead, weight.n)
+    if x.dtype not in _DTYPES:
+        raise TypeError('linear_i8 expects fp16, bf16, fp32 or Int8Rows, got %s' % x.dtype)
+    _refuse_grad('linear_i8', x)
+    if not x.is_cuda or x.numel() == 0:
+        return _plain_product(quantize_rows(x), weight, bias, act, slope, dtype).reshape(*x.shape[:-1], weight.n)
+    r, pitch = _rows_of(x)
+    return _linear(r, pitch, r.shape[0], weight, bias, act, slope, dtype).reshape(*x.shape[:-1], weight.n)
 
 
 def conv1x1_i8(x, weight, bias=None, act=None, slope=0.1, dtype=None):
@@ -208,16 +243,18 @@ def conv1x1_i8(x, weight, bias=None, act=None, slope=0.1, dtype=None):
         raise ValueError('conv1x1_i8 expects (batch, channels, ...), got %s' % (tuple(x.shape),))
     if x.dtype not in _DTYPES:
         raise TypeError('conv1x1_i8 expects fp16, bf16 or fp32, got %s' % x.dtype)
-    _refuse_grad('conv1x1_i8', x)
-    _check_k(x.shape[1])
     if not x.is_cuda or x.numel() == 0:
-        rows = quantize_rows(x.movedim(1, -1))
-    else:
-        pitch = pixel_pitch(x)
-        if pitch is None:
-            x, pitch = channels_last(x)
-        rows = _quantize(x, pitch, (x.shape[0], *x.shape[2:]), x.shape[1])
-    return linear_i8(rows, weight, bias, act, slope, dtype).movedim(-1, 1)
+        return linear_i8(x.movedim(1, -1), weight, bias, act, slope, dtype).movedim(-1, 1)
+    pitch = pixel_pitch(x)
+    if pitch is None:
+        return linear_i8(x.movedim(1, -1).contiguous(), weight, bias, act, slope, dtype).movedim(-1, 1)
+    dtype = dtype or x.dtype
+    bias = _check('conv1x1_i8', x, weight, bias, act, dtype)
+    if x.shape[1] != weight.k:
+        raise ValueError('%d channels, weights for %d' % (x.shape[1], weight.k))
+    _refuse_grad('conv1x1_i8', x)
+    y = _linear(x, pitch, x.numel() // weight.k, weight, bias, act, slope, dtype)
+    return y.reshape(x.shape[0], *x.shape[2:], weight.n).movedim(-1, 1)
 
 
 class Int8Linear(nn.Module):
