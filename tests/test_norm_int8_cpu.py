@@ -81,6 +81,15 @@ def test_refusals():
             call()
 
 
+def test_descriptors_filled_in_one_step():
+    v = list(range(1, 26))
+    d = _lib.group_norm_desc(*v)
+    assert [getattr(d, f[0]) for f in d._fields_] == v
+    v = list(range(1, 15))
+    d = _lib.gemm_i8_desc(*v)
+    assert [getattr(d, f[0]) for f in d._fields_] == v
+
+
 def _gn(**kw):
     base = dict(x=0x1000, y=0x2000, dy=0x3000, dx=0x4000, mean=0x5000, rstd=0x6000, workspace=0x10000, workspace_bytes=1 << 40, batch=2, pixels=9, c=16,
                 groups=4, x_ld=16, y_ld=16, dy_ld=16, dx_ld=16, eps=1e-5)

@@ -15,6 +15,7 @@ Channels: any number the groups divide, up to 4096 (multiples of 8; multiples of
 4096 / (8 / gcd(channels, 8)), e.g. 512 for odd counts in 16 bits.
 """
 import ctypes as C
+from functools import lru_cache
 
 import torch
 import torch.nn as nn
@@ -59,6 +60,8 @@ def pixel_pitch(x):
 
 def channels_last(x):
     """x itself where the kernels can walk it, else a channels_last copy; with its pixel pitch."""
+    if x.dim() == 4 and x.is_contiguous(memory_format=torch.channels_last):
+        return x, x.shape[1]
     pitch = pixel_pitch(x)
     if pitch is None or (pitch != x.shape[1] and x.shape[1] * x.element_size() % 16):
         x = x.movedim(1, -1).contiguous().movedim(-1, 1)
@@ -66,23 +69,15 @@ def channels_last(x):
     return x, pitch
 
 
-def empty_channels_last(shape, dtype, device):
-    return torch.empty((shape[0], *shape[2:], shape[1]), dtype=dtype, device=device).movedim(-1, 1)
+def empty_like_channels_last(x):
+    if x.dim() == 4 and x.is_contiguous(memory_format=torch.channels_last):
+        return torch.empty_like(x)
+    return torch.empty((x.shape[0], *x.shape[2:], x.shape[1]), dtype=x.dtype, device=x.device).movedim(-1, 1)
 
 
-class on_device:
-    """The launch context of a tensor: its device is current inside."""
-
-    def __init__(self, x):
-        self.guard = None if x.device.index == torch.cuda.current_device() else torch.cuda.device(x.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _current(x):
+    """Whether x's device is the current one."""
+    return x.device.index == torch.cuda.current_device()
 
 
 def _check(x, num_groups, weight, bias, eps, act):
@@ -117,69 +112,77 @@ def _plain(x, num_groups, weight, bias, eps, act, slope):
     return y.movedim(1, -1).contiguous().movedim(-1, 1)
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _desc(x, pitch, groups, weight, bias, eps, act, slope, y=None, dy=None, dy_ld=0, dx=None, dweight=None, dbias=None, mean=None, rstd=None):
-    p = weight if weight is not None else bias
-    n, c = x.shape[0], x.shape[1]
-    return _lib.GroupNormDesc(x.data_ptr(), _ptr(y), _ptr(dy), _ptr(dx), _ptr(weight), _ptr(bias), _ptr(dweight), _ptr(dbias),
-                              _ptr(mean), _ptr(rstd), None, 0, n, x.numel() // (n * c), c, groups, pitch, c, dy_ld, c,
-                              _DTYPES[x.dtype], _lib.F32 if p is None else _DTYPES[p.dtype], _ACTS[act], slope, eps)
-
-
-def _workspace(lib, d, what, device):
+@lru_cache(maxsize=4096)
+def _workspace_bytes(what, batch, pixels, c, groups, dtype, param_dtype):
+    d = _lib.group_norm_desc(*(0,) * 12, batch, pixels, c, groups, c, c, c, c, dtype, param_dtype, 0, 0.0, 0.0)
     n = C.c_size_t()
-    _lib.check(lib.y5_group_norm_workspace(C.byref(d), what, C.byref(n)))
-    if not n.value:
-        return None
-    ws = torch.empty(n.value, dtype=torch.uint8, device=device)
-    d.workspace, d.workspace_bytes = ws.data_ptr(), n.value
-    return ws
+    _lib.check(_lib.lib().y5_group_norm_workspace(C.byref(d), what, C.byref(n)))
+    return n.value
 
 
-def _forward(x, num_groups, weight, bias, eps, act, slope, stats):
-    """(y, mean, rstd, x as it was read, its pitch); mean and rstd where stats is true."""
-    with on_device(x):
-        lib = _lib.lib()
-        x, pitch = channels_last(x)
-        y = empty_channels_last(x.shape, x.dtype, x.device)
-        mean = rstd = None
-        if stats:
-            both = torch.empty((2, x.shape[0], num_groups), dtype=torch.float32, device=x.device)
-            mean, rstd = both[0], both[1]
-        d = _desc(x, pitch, num_groups, weight, bias, eps, act, slope, y=y, mean=mean, rstd=rstd)
-        ws = _workspace(lib, d, _lib.GN_FORWARD, x.device)  # noqa: F841 - held until the launch
-        _lib.check(lib.y5_group_norm(C.byref(d), _lib.current_stream()))
-    return y, mean, rstd, x
+def _run(what, x, pitch, groups, weight, bias, eps, act, slope, y=0, dy=0, dy_ld=0, dx=0, dweight=0, dbias=0, stats=0, rows=None):
+    """One of the three calls on x's (current) device and its current stream.  stats: address of (2, batch, groups) fp32."""
+    batch, c = x.shape[0], x.shape[1]
+    pixels = x.numel() // (batch * c)
+    p = weight if weight is not None else bias
+    dtype, param_dtype = _DTYPES[x.dtype], _lib.F32 if p is None else _DTYPES[p.dtype]
+    n = _workspace_bytes(what, batch, pixels, c, groups, dtype, param_dtype)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    d = _lib.group_norm_desc(x.data_ptr(), y, dy, dx, 0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                             dweight, dbias, stats, stats and stats + 4 * batch * groups, 0 if ws is None else ws.data_ptr(), n, batch, pixels, c,
+                             groups, pitch, c, dy_ld, c, dtype, param_dtype, _ACTS[act], slope, eps)
+    lib, stream = _lib.lib(), _lib.raw_stream(x.device.index)
+    if what == _lib.GN_FORWARD:
+        rc = lib.y5_group_norm(C.byref(d), stream)
+    elif what == _lib.GN_BACKWARD:
+        rc = lib.y5_group_norm_backward(C.byref(d), stream)
+    else:
+        rc = lib.y5_group_norm_rows_i8(C.byref(d), rows.q.data_ptr(), rows.q.shape[1], rows.scale.data_ptr(), stream)
+    if rc:
+        _lib.check(rc)
+
+
+def _forward(x, num_groups, weight, bias, eps, act, slope, want_stats):
+    """(y, x as it was read, (2, batch, groups) mean and 1 / deviation or None)."""
+    if not _current(x):
+        with torch.cuda.device(x.device):
+            return _forward(x, num_groups, weight, bias, eps, act, slope, want_stats)
+    x, pitch = channels_last(x)
+    y = empty_like_channels_last(x)
+    stats = torch.empty((2, x.shape[0], num_groups), dtype=torch.float32, device=x.device) if want_stats else None
+    _run(_lib.GN_FORWARD, x, pitch, num_groups, weight, bias, eps, act, slope, y=y.data_ptr(), stats=0 if stats is None else stats.data_ptr())
+    return y, x, stats
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, num_groups, eps, act, slope):
-        y, mean, rstd, xl = _forward(x, num_groups, weight, bias, eps, act, slope, True)
-        ctx.save_for_backward(xl, weight, bias, mean, rstd)
-        ctx.args = (num_groups, eps, act, slope)
+    def forward(ctx, x, weight, bias, *args):
+        y, xl, stats = _forward(x, args[0], weight, bias, *args[1:], True)
+        ctx.save_for_backward(xl, weight, bias, stats)
+        ctx.args = args
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        num_groups, eps, act, slope = ctx.args
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        with on_device(x):
-            lib = _lib.lib()
-            dy, dy_ld = channels_last(dy)
-            dx = empty_channels_last(x.shape, x.dtype, x.device) if need_x else None
-            dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_w else None
-            db = torch.empty_like(bias, memory_format=torch.contiguous_format) if need_b else None
-            d = _desc(x, pixel_pitch(x), num_groups, weight, bias, eps, act, slope, dy=dy, dy_ld=dy_ld, dx=dx, dweight=dw, dbias=db,
-                      mean=mean, rstd=rstd)
-            ws = _workspace(lib, d, _lib.GN_BACKWARD, x.device)  # noqa: F841 - held until the launch
-            _lib.check(lib.y5_group_norm_backward(C.byref(d), _lib.current_stream()))
-        return dx, dw, db, None, None, None, None
+        x, weight, bias, stats = ctx.saved_tensors
+        if not _current(x):
+            with torch.cuda.device(x.device):
+                return _backward(ctx, x, weight, bias, stats, dy)
+        return _backward(ctx, x, weight, bias, stats, dy)
+
+
+def _backward(ctx, x, weight, bias, stats, dy):
+    need = ctx.needs_input_grad
+    dy, dy_ld = channels_last(dy)
+    dx = empty_like_channels_last(x) if need[0] else None
+    dw = torch.empty_like(weight) if need[1] else None
+    db = torch.empty_like(bias) if need[2] else None
+    num_groups, eps, act, slope = ctx.args
+    _run(_lib.GN_BACKWARD, x, channels_last(x)[1], num_groups, weight, bias, eps, act, slope, dy=dy.data_ptr(), dy_ld=dy_ld,
+         dx=0 if dx is None else dx.data_ptr(), dweight=0 if dw is None else dw.data_ptr(), dbias=0 if db is None else db.data_ptr(),
+         stats=stats.data_ptr())
+    return dx, dw, db, None, None, None, None
 
 
 def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, slope=0.1):
@@ -189,8 +192,10 @@ def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, slope=
     _check(x, num_groups, weight, bias, eps, act)
     if not x.is_cuda or x.numel() == 0:
         return _plain(x, num_groups, weight, bias, eps, act, slope)
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         return _GroupNorm.apply(x, weight, bias, num_groups, eps, act, slope)
     return _forward(x, num_groups, weight, bias, eps, act, slope, False)[0]
@@ -212,13 +217,12 @@ def group_norm_rows(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, s
         return rows
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    with on_device(x):
-        lib = _lib.lib()
-        x, pitch = channels_last(x)
-        rows = int8.Int8Rows.empty(lead, x.shape[1], x.dtype, x.device)
-        d = _desc(x, pitch, num_groups, weight, bias, eps, act, slope)
-        ws = _workspace(lib, d, _lib.GN_ROWS, x.device)  # noqa: F841 - held until the launch
-        _lib.check(lib.y5_group_norm_rows_i8(C.byref(d), rows.q.data_ptr(), rows.q.shape[1], rows.scale.data_ptr(), _lib.current_stream()))
+    if not _current(x):
+        with torch.cuda.device(x.device):
+            return group_norm_rows(x, num_groups, weight, bias, eps, act, slope)
+    x, pitch = channels_last(x)
+    rows = int8.Int8Rows.empty(lead, x.shape[1], x.dtype, x.device)
+    _run(_lib.GN_ROWS, x, pitch, num_groups, weight, bias, eps, act, slope, rows=rows)
     return rows
 
 

@@ -14,12 +14,13 @@ A row x becomes whole numbers q = nearest(127 x / max|x|) and the scale max|x| /
 Inference only.  CPU tensors go through torch's own operators (sums in fp64, exact too).
 """
 import ctypes as C
+from functools import lru_cache
 
 import torch
 import torch.nn as nn
 
 from yolo_amd import _lib
-from yolo_amd.groupnorm import _ACTS, _DTYPES, act_code, apply_act, on_device, pixel_pitch
+from yolo_amd.groupnorm import _ACTS, _DTYPES, _current, act_code, apply_act, pixel_pitch
 
 ZERO_ROW = 2.0 ** -120
 
@@ -113,10 +114,12 @@ def _quantize_plain(x, lead, k, dtype):
 
 def _quantize(x, pitch, lead, k):
     """x: any view whose rows of k values lie `pitch` elements apart."""
-    with on_device(x):
-        rows = Int8Rows.empty(lead, k, x.dtype, x.device)
-        _lib.check(_lib.lib().y5_quantize_rows_i8(x.data_ptr(), pitch, _DTYPES[x.dtype], rows.q.shape[0], k, rows.q.data_ptr(),
-                                                  rows.q.shape[1], rows.scale.data_ptr(), _lib.current_stream()))
+    if not _current(x):
+        with torch.cuda.device(x.device):
+            return _quantize(x, pitch, lead, k)
+    rows = Int8Rows.empty(lead, k, x.dtype, x.device)
+    _lib.check(_lib.lib().y5_quantize_rows_i8(x.data_ptr(), pitch, _DTYPES[x.dtype], rows.q.shape[0], k, rows.q.data_ptr(),
+                                              rows.q.shape[1], rows.scale.data_ptr(), _lib.raw_stream(x.device.index)))
     return rows
 
 
@@ -162,34 +165,49 @@ def _plain_product(rows, weight, bias, act, slope, dtype):
     return apply_act(y, act, slope).to(dtype)
 
 
-def _desc(rows, weight, bias, act, slope, y, m):
-    return _lib.GemmI8Desc(None if rows is None else rows.q.data_ptr(), None if rows is None else rows.scale.data_ptr(), weight.q.data_ptr(),
-                           weight.scale.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), m, weight.n, weight.n, weight.k,
-                           weight.q.shape[1], _DTYPES[y.dtype], _ACTS[act], slope)
+def _desc(q, scale, weight, bias, act, slope, y, m):
+    return _lib.gemm_i8_desc(q, scale, weight.q.data_ptr(), weight.scale.data_ptr(), 0 if bias is None else bias.data_ptr(), y.data_ptr(), m,
+                             weight.n, weight.n, weight.k, weight.q.shape[1], _DTYPES[y.dtype], _ACTS[act], slope)
 
 
 def _product(rows, weight, bias, act, slope, dtype):
     """(rows, n) of dtype from Int8Rows."""
-    m = rows.q.shape[0]
-    if not rows.q.is_cuda or m == 0:
+    q = rows.q
+    m = q.shape[0]
+    if not q.is_cuda or m == 0:
         return _plain_product(rows, weight, bias, act, slope, dtype)
-    with on_device(rows.q):
-        y = torch.empty((m, weight.n), dtype=dtype, device=rows.q.device)
-        _lib.check(_lib.lib().y5_gemm_i8(C.byref(_desc(rows, weight, bias, act, slope, y, m)), _lib.current_stream()))
+    if not _current(q):
+        with torch.cuda.device(q.device):
+            return _product(rows, weight, bias, act, slope, dtype)
+    y = torch.empty((m, weight.n), dtype=dtype, device=q.device)
+    d = _desc(q.data_ptr(), rows.scale.data_ptr(), weight, bias, act, slope, y, m)
+    rc = _lib.lib().y5_gemm_i8(C.byref(d), _lib.raw_stream(q.device.index))
+    if rc:
+        _lib.check(rc)
     return y
+
+
+@lru_cache(maxsize=4096)
+def _workspace_bytes(m, n, k, dtype, x_dtype):
+    d = _lib.gemm_i8_desc(0, 0, 0, 0, 0, 0, m, n, n, k, row_bytes(k), dtype, 0, 0.0)
+    size = C.c_size_t()
+    _lib.check(_lib.lib().y5_linear_i8_workspace(C.byref(d), x_dtype, C.byref(size)))
+    return size.value
 
 
 def _linear(x, pitch, m, weight, bias, act, slope, dtype):
     """(m, n) of dtype from m rows `pitch` elements apart, quantised on the way."""
-    with on_device(x):
-        lib = _lib.lib()
-        y = torch.empty((m, weight.n), dtype=dtype, device=x.device)
-        d = _desc(None, weight, bias, act, slope, y, m)
-        n = C.c_size_t()
-        _lib.check(lib.y5_linear_i8_workspace(C.byref(d), _DTYPES[x.dtype], C.byref(n)))
-        ws = torch.empty(n.value, dtype=torch.uint8, device=x.device) if n.value else None
-        _lib.check(lib.y5_linear_i8(C.byref(d), x.data_ptr(), pitch, _DTYPES[x.dtype], None if ws is None else ws.data_ptr(), n.value,
-                                    _lib.current_stream()))
+    if not _current(x):
+        with torch.cuda.device(x.device):
+            return _linear(x, pitch, m, weight, bias, act, slope, dtype)
+    y = torch.empty((m, weight.n), dtype=dtype, device=x.device)
+    d = _desc(0, 0, weight, bias, act, slope, y, m)
+    x_dtype = _DTYPES[x.dtype]
+    n = _workspace_bytes(m, weight.n, weight.k, _DTYPES[dtype], x_dtype)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    rc = _lib.lib().y5_linear_i8(C.byref(d), x.data_ptr(), pitch, x_dtype, None if ws is None else ws.data_ptr(), n, _lib.raw_stream(x.device.index))
+    if rc:
+        _lib.check(rc)
     return y
 
 
@@ -207,8 +225,9 @@ def _check(name, x, weight, bias, act, dtype):
         raise ValueError('bias must be %d floating-point values, got %s %s' % (weight.n, tuple(bias.shape), bias.dtype))
     if bias.device != weight.device:
         raise ValueError('bias is on %s, the weight on %s' % (bias.device, weight.device))
-    _refuse_grad(name, bias)
-    return bias.float().contiguous()
+    if bias.requires_grad:
+        _refuse_grad(name, bias)
+    return bias if bias.dtype is torch.float32 and bias.is_contiguous() else bias.float().contiguous()
 
 
 def linear_i8(x, weight, bias=None, act=None, slope=0.1, dtype=None):
@@ -225,11 +244,13 @@ def linear_i8(x, weight, bias=None, act=None, slope=0.1, dtype=None):
         return _product(x, weight, bias, act, slope, dtype).reshape(*x.lead, weight.n)
     if x.dtype not in _DTYPES:
         raise TypeError('linear_i8 expects fp16, bf16, fp32 or Int8Rows, got %s' % x.dtype)
-    _refuse_grad('linear_i8', x)
+    if x.requires_grad:
+        _refuse_grad('linear_i8', x)
     if not x.is_cuda or x.numel() == 0:
         return _plain_product(quantize_rows(x), weight, bias, act, slope, dtype).reshape(*x.shape[:-1], weight.n)
     r, pitch = _rows_of(x)
-    return _linear(r, pitch, r.shape[0], weight, bias, act, slope, dtype).reshape(*x.shape[:-1], weight.n)
+    y = _linear(r, pitch, r.shape[0], weight, bias, act, slope, dtype)
+    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.n)
 
 
 def conv1x1_i8(x, weight, bias=None, act=None, slope=0.1, dtype=None):
