@@ -301,7 +301,7 @@ struct PhTile {
     int bm, bn;
     float round, ktile;
 };
-constexpr PhTile kPhTiles[] = {{256, 256, 6.f, 1.4f}, {256, 128, 4.f, 0.85f}, {128, 128, 2.5f, 0.6f}, {128, 64, 2.f, 0.45f}};
+constexpr PhTile kPhTiles[] = {{256, 256, 6.5f, 1.4f}, {256, 128, 3.5f, 0.85f}, {128, 128, 2.5f, 0.6f}, {128, 64, 2.f, 0.45f}};
 constexpr float kPhLaunch = 2.f;
 
 float ph_cost(const GemmArgs& g, const PhTile& p) {

@@ -38,10 +38,7 @@ __device__ __forceinline__ void quantise_to_lds(const FewArgs& a, unsigned char*
 #pragma unroll
             for (int e = 0; e < V; ++e) top = max_bits(top, (float)v[e]);
         }
-        for (int d = 32; d; d >>= 1) {
-            const unsigned o = (unsigned)__shfl_xor((int)top, d);
-            top = o > top ? o : top;
-        }
+        top = max_over(top, 64);
         if ((t & 63) == 0) atomicMax(&tops[r], top);  // the same whatever the order
     }
     __syncthreads();
@@ -58,11 +55,11 @@ __device__ __forceinline__ void quantise_to_lds(const FewArgs& a, unsigned char*
             TI v[V];
             if (a.k - k >= V) ld_vec(x + k, v);
             else ld_part(x + k, a.k - k, v);
-            int w[V];
+            unsigned w[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) w[e] = fine ? inv((float)v[e]) : 0;
+            for (int e = 0; e < V; ++e) w[e] = inv((float)v[e]);
 #pragma unroll
-            for (int e = 0; e < V; e += 4) *reinterpret_cast<int*>(q + r * a.g.ld + k + e) = pack_bytes(w[e], w[e + 1], w[e + 2], w[e + 3]);
+            for (int e = 0; e < V; e += 4) *reinterpret_cast<int*>(q + r * a.g.ld + k + e) = pack_bytes(w[e], w[e + 1], w[e + 2], w[e + 3], fine);
         }
     }
     __syncthreads();

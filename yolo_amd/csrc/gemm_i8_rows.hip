@@ -102,11 +102,7 @@ __global__ __launch_bounds__(512, 2) void gemm_rows_kernel(const RowsGemm a) {
                     for (int u = 0; u < Frag<TX>::NV; ++u)
 #pragma unroll
                         for (int e = 0; e < NormElem<TX>::V; ++e) top = max_bits(top, (float)raw[i][f].v[u][e]);
-#pragma unroll
-                for (int d = 16; d <= 32; d *= 2) {
-                    const unsigned o = (unsigned)__shfl_xor((int)top, d);
-                    top = o > top ? o : top;
-                }
+                top = max_over<16>(top, 64);  // of the four lanes that share a row
                 const bool fine = top < 0x7f800000u;
                 float m;
                 s[i] = row_scale(top, &m);
@@ -114,13 +110,13 @@ __global__ __launch_bounds__(512, 2) void gemm_rows_kernel(const RowsGemm a) {
                 inv.set(m, fine);
 #pragma unroll
                 for (int f = 0; f < KF; ++f) {
-                    int w[16];
+                    unsigned w[16];
 #pragma unroll
                     for (int u = 0; u < Frag<TX>::NV; ++u)
 #pragma unroll
                         for (int e = 0; e < NormElem<TX>::V; ++e) w[u * NormElem<TX>::V + e] = inv((float)raw[i][f].v[u][e]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) q[i][f][e] = fine ? pack_bytes(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]) : 0;
+                    for (int e = 0; e < 4; ++e) q[i][f][e] = pack_bytes(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3], fine);
                 }
             } else {
                 s[i] = sn[i];

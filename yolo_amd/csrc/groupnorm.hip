@@ -18,12 +18,13 @@
 
 namespace {
 
+#include "conv_common.h"
 #include "norm_rows.h"
 
 struct GnArgs {
     NormShape s;
     const void *x, *dy, *weight, *bias;
-    void *y, *dx;
+    void *y, *dx, *dweight, *dbias;
     float *mean, *rstd;  // [batch][groups]
     float2* part;        // [batch][chunks][groups]: a chunk's statistics (forward) or its S1, S2 (backward)
     float* cpart;        // backward: [batch * chunks][2][c], a chunk's sums of dz and of dz * xh
@@ -64,123 +65,173 @@ __device__ __forceinline__ void col_sum(float (&v)[N], int j, int r, int RT, int
     __syncthreads();
 }
 
-// f(g, sum) for the G groups from g0 on, sum = sum over the group's entries of at(entry): entries rep * rep_pitch + g * n + i
-// for rep < reps, i < n.  A thread a group, or a wave where a group has many entries.
+// f(g, sums) for G groups, sums = the sums over the group's entries of at(entry), two at a time: entries rep * rep_pitch + g * n + i for
+// rep < reps, i < n.  A thread a group, or a wave where a group has many entries.
 template <typename At, typename F>
-__device__ __forceinline__ void group_sum(int G, int n, int reps, int rep_pitch, At at, F f) {
+__device__ __forceinline__ void group_sum2(int G, int n, int reps, int rep_pitch, At at, F f) {
     const int t = threadIdx.x, T = blockDim.x;
     if (n * reps <= 32) {
         for (int g = t; g < G; g += T) {
-            float a = 0.f;
+            float2 a = make_float2(0.f, 0.f);
             for (int k = 0; k < reps; ++k)
-                for (int i = 0; i < n; ++i) a += at(k * rep_pitch + g * n + i);
+                for (int i = 0; i < n; ++i) {
+                    const float2 v = at(k * rep_pitch + g * n + i);
+                    a.x += v.x;
+                    a.y += v.y;
+                }
             f(g, a);
         }
     } else {
         const int lane = t & 63;
         for (int g = t >> 6; g < G; g += T >> 6) {
-            float a = 0.f;
+            float2 a = make_float2(0.f, 0.f);
             for (int k = 0; k < reps; ++k)
-                for (int i = lane; i < n; i += 64) a += at(k * rep_pitch + g * n + i);
-            for (int off = 32; off; off >>= 1) a += __shfl_xor(a, off);
+                for (int i = lane; i < n; i += 64) {
+                    const float2 v = at(k * rep_pitch + g * n + i);
+                    a.x += v.x;
+                    a.y += v.y;
+                }
+            for (int off = 32; off; off >>= 1) {
+                a.x += __shfl_xor(a.x, off);
+                a.y += __shfl_xor(a.y, off);
+            }
             if (lane == 0) f(g, a);
         }
     }
     __syncthreads();
 }
 
+// How the elements of a vector lie to groups and rows: all of one group; each of a group of its own (a group is no multiple of a
+// vector); each of a group of its own in virtual rows of several pixels, the last of which may be cut short
+enum { kUniform, kMixed, kCut };
+
 // The vector column a thread owns: element offset in the virtual row, channels, groups and parameters of its elements.
-// PER: every element may belong to another group (a group is no multiple of a vector, or a virtual row is several pixels).
-template <typename T, bool PER>
+template <typename T, int M>
 struct Column {
-    static constexpr int V = NormElem<T>::V, NG = PER ? V : 1;
+    static constexpr int V = NormElem<T>::V, NG = M ? V : 1;
     int off;      // element offset of the vector in the virtual row
     int ch0;      // channel of its first element
     int grp[NG];  // group of each element
     __device__ __forceinline__ void init(const NormShape& s, int col) {
         off = col * V;
-        ch0 = s.k == 1 ? off : off % s.c;
-        if (PER) {
+        ch0 = M == kCut ? mod_c(s, off) : off;
+        if (M) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) grp[e] = channel(s, e) / s.cpg;
+            for (int e = 0; e < V; ++e) grp[e] = (int)fdiv((unsigned)channel(s, e), s.by_cpg);
         } else {
-            grp[0] = off / s.cpg;
+            grp[0] = (int)fdiv((unsigned)off, s.by_cpg);
         }
     }
     __device__ __forceinline__ int channel(const NormShape& s, int e) const {
         const int c = ch0 + e;  // below s.c + V: a virtual row of narrow pixels may hold several of them in one vector
-        return PER && c >= s.c ? c % s.c : c;
+        return M == kCut ? mod_c(s, c) : c;
+    }
+    static __device__ __forceinline__ int mod_c(const NormShape& s, int i) { return i - (int)fdiv((unsigned)i, s.by_c) * s.c; }
+    // a parameter vector's values for the elements
+    __device__ __forceinline__ void params(const NormShape& s, const void* p, float def, float (&v)[V]) const {
+        if constexpr (M == kCut) {
+            if (!p || s.param_dtype == Y5_F32) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[e] = p ? static_cast<const float*>(p)[channel(s, e)] : def;
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const unsigned short b = static_cast<const unsigned short*>(p)[channel(s, e)];
+                    v[e] = s.param_dtype == Y5_F16 ? (float)__builtin_bit_cast(f16, b) : __uint_as_float((unsigned)b << 16);
+                }
+            }
+        } else {
+            ld_params(p, ch0, s.param_dtype, def, v);
+        }
     }
     // elements of the vector that virtual row `row` has
     __device__ __forceinline__ int valid(const NormShape& s, int row) const {
-        if (!PER || s.k == 1) return V;
+        if (M != kCut) return V;
         const long long left = (long long)s.pixels * s.c - ((long long)row * s.W + off);
         return left >= V ? V : left > 0 ? (int)left : 0;
     }
 };
 
-template <typename T, bool PER>
-__device__ __forceinline__ void ld_col(const T* p, int nv, T (&v)[NormElem<T>::V]) {
-    if (!PER || nv >= NormElem<T>::V) ld_vec(p, v);
-    else ld_part(p, nv, v);
+// A vector of T as the 16 bytes it is in memory: what is kept across a barrier stays packed.
+typedef norm_u32x4 Raw;
+template <typename T, int M>
+__device__ __forceinline__ Raw ld_col(const T* p, int nv) {
+    if (M != kCut || nv >= NormElem<T>::V) return reinterpret_cast<const NormVec<T>*>(p)->v;
+    NormArr<T> u;
+    ld_part(p, nv, u.v);
+    return __builtin_bit_cast(Raw, u);
 }
-template <typename T, bool PER>
-__device__ __forceinline__ void st_col(T* p, int nv, const T (&v)[NormElem<T>::V]) {
-    if (!PER || nv >= NormElem<T>::V) st_vec(p, v);
-    else st_part(p, nv, v);
+// its elements; the empty statement keeps the compiler from unpacking it where it was loaded, or once for every use
+template <typename T>
+__device__ __forceinline__ NormArr<T> unpack(Raw& r) {
+    asm volatile("" : "+v"(r));
+    return __builtin_bit_cast(NormArr<T>, r);
+}
+template <typename T, int M>
+__device__ __forceinline__ void st_col(T* p, int nv, const Raw& r) {
+    if (M != kCut || nv >= NormElem<T>::V) reinterpret_cast<NormVec<T>*>(p)->v = r;
+    else st_part(p, nv, __builtin_bit_cast(NormArr<T>, r).v);
 }
 
 // z = act(gamma (x - mean) rstd + beta) of one vector, rounded once
-template <typename T, int NG>
-__device__ __forceinline__ void normalise(const T (&in)[NormElem<T>::V], T (&out)[NormElem<T>::V], const float (&mean)[NG],
-                                          const float (&A)[NormElem<T>::V], const float (&B)[NormElem<T>::V], int act, float slope) {
+template <typename T, bool SILU, int NG>
+__device__ __forceinline__ Raw normalise(Raw& raw, const float (&mean)[NG], const float (&A)[NormElem<T>::V], const float (&B)[NormElem<T>::V],
+                                         float slope) {
     constexpr int V = NormElem<T>::V;
+    const NormArr<T> in = unpack<T>(raw);
+    NormArr<T> out;
     float z[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) z[e] = __builtin_fmaf((float)in[e] - mean[NG == 1 ? 0 : e], A[e], B[e]);
-    norm_act(z, act, slope);
+    for (int e = 0; e < V; ++e) z[e] = __builtin_fmaf((float)in.v[e] - mean[NG == 1 ? 0 : e], A[e], B[e]);
+    norm_act<SILU>(z, slope);
 #pragma unroll
-    for (int e = 0; e < V; ++e) out[e] = (T)z[e];
+    for (int e = 0; e < V; ++e) out.v[e] = (T)z[e];
+    return __builtin_bit_cast(Raw, out);
 }
 
 // ------------------------------------------------------------------------------------------ forward, resident
 
-// grid (slices, batch).  LDS: part[blockDim.x * NG], tot[cols * NG], gs[2 * groups of the slice]
-template <typename T, bool PER, int R>
-__global__ __launch_bounds__(R > 8 ? 1024 : R > 4 ? 512 : 256) void gn_resident_kernel(const GnArgs a, int cols) {
-    constexpr int V = NormElem<T>::V, NG = PER ? V : 1;
+// grid: slices * batch.  LDS: part[blockDim.x * NG], tot[cols * NG], gs[2 * groups of the slice]
+template <typename T, int M, bool SILU, int R>
+__global__ __launch_bounds__(R > 8 ? 1024 : R > 4 ? 512 : 256, 4) void gn_resident_kernel(const GnArgs a, const FastDiv by_cols, int slices) {
+    constexpr int V = NormElem<T>::V, NG = M ? V : 1;
     extern __shared__ float lds[];
     const NormShape& s = a.s;
-    const int t = threadIdx.x, TB = blockDim.x, b = blockIdx.y;
-    const int RT = TB / cols, r = t / cols, j = t - r * cols;
+    // slices of an image share cache lines: neighbours run on one XCD, behind one L2
+    const int at = xcd_remap(blockIdx.x, gridDim.x), b = at / slices, slice = at - b * slices;
+    const int t = threadIdx.x, TB = blockDim.x, cols = (int)by_cols.d;
+    const int RT = (int)fdiv((unsigned)TB, by_cols), r = (int)fdiv((unsigned)t, by_cols), j = t - r * cols;
     const bool active = r < RT;
     float *part = lds, *tot = part + TB * NG, *gs = tot + cols * NG;
-    Column<T, PER> col;
-    col.init(s, blockIdx.x * cols + j);
-    const int g0 = blockIdx.x * cols * V / s.cpg;                  // first group of the slice (a slice holds whole groups)
-    const int G = PER && s.k > 1 ? s.groups : cols * V / s.cpg;    // its groups
-    const int gn = PER ? s.cpg : s.cpg / V;                        // entries of a group in tot
+    Column<T, M> col;
+    col.init(s, slice * cols + j);
+    const int g0 = (int)fdiv(slice * cols * V, s.by_cpg);  // first group of the slice (a slice holds whole groups)
+    const int G = M == kCut ? s.groups : (int)fdiv(cols * V, s.by_cpg);  // its groups
+    const int gn = M ? s.cpg : s.cpg / V;                        // entries of a group in tot
     const T* xb = static_cast<const T*>(a.x) + (size_t)b * a.x_img + col.off;
-    T raw[R][V];
-    int nv[R];
+    Raw raw[R];
+    auto valid = [&](int i) { return active && r + i * RT < s.vrows ? col.valid(s, r + i * RT) : 0; };
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        const int row = r + i * RT;
-        nv[i] = active && row < s.vrows ? col.valid(s, row) : 0;
-        if (nv[i]) ld_col<T, PER>(xb + (size_t)row * a.x_row, nv[i], raw[i]);
+        const int nv = valid(i);
+        if (nv) raw[i] = ld_col<T, M>(xb + (size_t)(r + i * RT) * a.x_row, nv);
     }
+    float A[V], B[V];  // gamma (times 1 / deviation, later) and beta: on their way with the values
+    col.params(s, a.weight, 1.f, A);
+    col.params(s, a.bias, 0.f, B);
     float acc[NG];
 #pragma unroll
     for (int e = 0; e < NG; ++e) acc[e] = 0.f;
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (nv[i]) {
+        if (valid(i)) {
+            const NormArr<T> x = unpack<T>(raw[i]);
 #pragma unroll
-            for (int e = 0; e < V; ++e) acc[PER ? e : 0] += (float)raw[i][e];
+            for (int e = 0; e < V; ++e) acc[M ? e : 0] += (float)x.v[e];
         }
     const float inv_n = 1.f / ((float)s.pixels * (float)s.cpg);
     col_sum<NG>(acc, j, r, RT, cols, part, tot);
-    group_sum(G, gn, s.k, s.c, [&](int i) { return tot[i]; }, [&](int g, float v) { gs[2 * g] = v * inv_n; });
+    group_sum2(G, gn, s.k, s.c, [&](int i) { return make_float2(tot[i], 0.f); }, [&](int g, float2 v) { gs[2 * g] = v.x * inv_n; });
     float mean[NG];
 #pragma unroll
     for (int e = 0; e < NG; ++e) {
@@ -189,15 +240,16 @@ __global__ __launch_bounds__(R > 8 ? 1024 : R > 4 ? 512 : 256) void gn_resident_
     }
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (nv[i]) {
+        if (const int nv = valid(i)) {
+            const NormArr<T> x = unpack<T>(raw[i]);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float d = (float)raw[i][e] - mean[PER ? e : 0];
-                if (!PER || e < nv[i]) acc[PER ? e : 0] = __builtin_fmaf(d, d, acc[PER ? e : 0]);
+                const float d = (float)x.v[e] - mean[M ? e : 0];
+                if (M != kCut || e < nv) acc[M ? e : 0] = __builtin_fmaf(d, d, acc[M ? e : 0]);
             }
         }
     col_sum<NG>(acc, j, r, RT, cols, part, tot);
-    group_sum(G, gn, s.k, s.c, [&](int i) { return tot[i]; }, [&](int g, float v) { gs[2 * g + 1] = 1.f / sqrtf(v * inv_n + s.eps); });
+    group_sum2(G, gn, s.k, s.c, [&](int i) { return make_float2(tot[i], 0.f); }, [&](int g, float2 v) { gs[2 * g + 1] = 1.f / sqrtf(v.x * inv_n + s.eps); });
     if (a.mean) {
         for (int g = t; g < G; g += TB) {
             a.mean[(size_t)b * s.groups + g0 + g] = gs[2 * g];
@@ -205,37 +257,29 @@ __global__ __launch_bounds__(R > 8 ? 1024 : R > 4 ? 512 : 256) void gn_resident_
         }
     }
     if (!active) return;
-    float A[V], B[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-        const int c = col.channel(s, e);
-        A[e] = ld_param(a.weight, c, s.param_dtype, 1.f) * gs[2 * (col.grp[PER ? e : 0] - g0) + 1];
-        B[e] = ld_param(a.bias, c, s.param_dtype, 0.f);
-    }
+    for (int e = 0; e < V; ++e) A[e] *= gs[2 * (col.grp[M ? e : 0] - g0) + 1];
     T* yb = static_cast<T*>(a.y) + (size_t)b * a.y_img + col.off;
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (nv[i]) {
-            T out[V];
-            normalise<T, NG>(raw[i], out, mean, A, B, s.act, s.slope);
-            st_col<T, PER>(yb + (size_t)(r + i * RT) * a.y_row, nv[i], out);
-        }
+        if (const int nv = valid(i)) st_col<T, M>(yb + (size_t)(r + i * RT) * a.y_row, nv, normalise<T, SILU, NG>(raw[i], mean, A, B, s.slope));
 }
 
 // ------------------------------------------------------------------------------------------ forward, split
 
-// grid (chunks, batch): (mean, M2) of every group over the chunk.  A thread sums differences from the first value it reads
-// (K): where a map's mean is many deviations from zero, sum and sum of squares of the raw values would cancel.
-template <typename T, bool PER>
-__global__ __launch_bounds__(1024) void gn_stats_kernel(const GnArgs a) {
-    constexpr int V = NormElem<T>::V, NG = PER ? V : 1, NA = PER ? V : 4;
+// grid (chunks, batch): (mean, M2) of every group over the chunk.  A thread sums differences from the first value it reads (K):
+// where a map's mean is many deviations from zero, sum and sum of squares of the raw values would cancel.  The threads' means and
+// squares then meet as differences from one thread's mean of each group.
+template <typename T, int M>
+__global__ __launch_bounds__(1024, sizeof(T) == 4 || M == kUniform ? 8 : 6) void gn_stats_kernel(const GnArgs a) {
+    constexpr int V = NormElem<T>::V, NG = M ? V : 1, NA = M ? V : 4;
     extern __shared__ float lds[];
     const NormShape& s = a.s;
     const int t = threadIdx.x, TB = blockDim.x, b = blockIdx.y, cols = s.cols;
-    const int RT = TB / cols, r = t / cols, j = t - r * cols;
+    const int RT = (int)fdiv((unsigned)TB, s.by_cols), r = (int)fdiv((unsigned)t, s.by_cols), j = t - r * cols;
     const bool active = r < RT;
-    float *part = lds, *tot = part + TB * NG, *gs = tot + cols * NG;
-    Column<T, PER> col;
+    float *part = lds, *tot = part + TB * 2 * NG, *gs = tot + cols * 2 * NG;
+    Column<T, M> col;
     col.init(s, j);
     const int row0 = blockIdx.x * s.chunk_rows;
     const int row1 = row0 + s.chunk_rows < s.vrows ? row0 + s.chunk_rows : s.vrows;
@@ -248,82 +292,103 @@ __global__ __launch_bounds__(1024) void gn_stats_kernel(const GnArgs a) {
     if (active && row0 + r < row1) {
         int row = row0 + r;
         {
-            T v[V];
-            const int nv = col.valid(s, row);
-            ld_col<T, PER>(xb + (size_t)row * a.x_row, nv, v);
+            Raw raw = ld_col<T, M>(xb + (size_t)row * a.x_row, col.valid(s, row));
+            const NormArr<T> v = unpack<T>(raw);
 #pragma unroll
-            for (int e = 0; e < NG; ++e) K[e] = (float)v[e];
+            for (int e = 0; e < NG; ++e) K[e] = (float)v.v[e];
         }
-        auto take = [&](const T (&v)[V], int nv) {
+        auto take = [&](Raw& raw, int nv) {
+            const NormArr<T> v = unpack<T>(raw);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float d = (float)v[e] - K[PER ? e : 0];
-                if (!PER || e < nv) {
+                const float d = (float)v.v[e] - K[M ? e : 0];
+                if (M != kCut || e < nv) {
                     S[e % NA] += d;
                     Q[e % NA] = __builtin_fmaf(d, d, Q[e % NA]);
-                    if (PER) n[e] += 1.f;
+                    if (M == kCut) n[e] += 1.f;
                 }
             }
-            if (!PER) n[0] += (float)V;
         };
         const long long step = (long long)RT * a.x_row;
         const T* p = xb + (size_t)row * a.x_row;
         // four loads in flight; the last row of an image may be cut short and is left to the loop behind
-        for (; row + 3 * RT < row1 - (PER ? 1 : 0); row += 4 * RT, p += 4 * step) {
-            T v[4][V];
+        for (; row + 3 * RT < row1 - (M == kCut ? 1 : 0); row += 4 * RT, p += 4 * step) {
+            Raw v[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) ld_vec(p + u * step, v[u]);
+            for (int u = 0; u < 4; ++u) v[u] = ld_col<T, M>(p + u * step, V);
 #pragma unroll
             for (int u = 0; u < 4; ++u) take(v[u], V);
         }
         for (; row < row1; row += RT, p += step) {
-            T v[V];
             const int nv = col.valid(s, row);
-            ld_col<T, PER>(p, nv, v);
+            Raw v = ld_col<T, M>(p, nv);
             take(v, nv);
+        }
+        if (M != kCut) {
+            const float rows = (float)((row1 - 1 - row0 - r) / RT + 1);
+#pragma unroll
+            for (int e = 0; e < NG; ++e) n[e] = M ? rows : rows * V;
         }
     }
     float m[NG], q[NG];
-    if (PER) {
-#pragma unroll
-        for (int e = 0; e < NG; ++e) {
-            const float d = n[e] > 0.f ? S[e] / n[e] : 0.f;
-            m[e] = K[e] + d;
-            q[e] = Q[e] - S[e] * d;
-        }
-    } else {
-        const float sum = (S[0] + S[1]) + (S[2] + S[3]), sq = (Q[0] + Q[1]) + (Q[2] + Q[3]);
-        const float d = n[0] > 0.f ? sum / n[0] : 0.f;
-        m[0] = K[0] + d;
-        q[0] = sq - sum * d;
-    }
-    const int G = s.groups, gn = PER ? s.cpg : s.cpg / V;
-    const float inv_n = 1.f / ((float)norm_chunk_pixels(s, blockIdx.x) * (float)s.cpg);
-    float acc[NG];
-#pragma unroll
-    for (int e = 0; e < NG; ++e) acc[e] = n[e] > 0.f ? n[e] * m[e] : 0.f;
-    col_sum<NG>(acc, j, r, RT, cols, part, tot);
-    group_sum(G, gn, s.k, s.c, [&](int i) { return tot[i]; }, [&](int g, float v) { gs[g] = v * inv_n; });
 #pragma unroll
     for (int e = 0; e < NG; ++e) {
-        const float d = active ? m[e] - gs[col.grp[e]] : 0.f;
-        acc[e] = n[e] > 0.f ? __builtin_fmaf(n[e] * d, d, q[e]) : 0.f;
+        const float sum = M ? S[e] : (S[0] + S[1]) + (S[2] + S[3]), sq = M ? Q[e] : (Q[0] + Q[1]) + (Q[2] + Q[3]);
+        const float d = n[e] > 0.f ? sum / n[e] : 0.f;
+        m[e] = K[e] + d;
+        q[e] = sq - sum * d;
     }
-    col_sum<NG>(acc, j, r, RT, cols, part, tot);
+    // the reference of a group: the mean that the first row's thread of its first element has (element g * cpg of a chunk's first
+    // virtual row is always there)
+    const int G = s.groups, gn = M ? s.cpg : s.cpg / V;
+    if (r == 0) {
+#pragma unroll
+        for (int e = 0; e < NG; ++e)
+            if (col.off + e < s.c && col.grp[e] * s.cpg == col.off + e) gs[col.grp[e]] = m[e];
+    }
+    __syncthreads();
+    float acc[2 * NG];
+#pragma unroll
+    for (int e = 0; e < NG; ++e) {
+        const float d = m[e] - gs[col.grp[e]];
+        acc[2 * e] = n[e] > 0.f ? n[e] * d : 0.f;
+        acc[2 * e + 1] = n[e] > 0.f ? __builtin_fmaf(n[e] * d, d, q[e]) : 0.f;
+    }
+    col_sum<2 * NG>(acc, j, r, RT, cols, part, tot);
     float2* out = a.part + ((size_t)b * s.chunks + blockIdx.x) * s.groups;
-    group_sum(G, gn, s.k, s.c, [&](int i) { return tot[i]; }, [&](int g, float v) { out[g] = make_float2(gs[g], v); });
+    const float N = (float)norm_chunk_pixels(s, blockIdx.x) * (float)s.cpg;
+    group_sum2(G, gn, s.k, s.c, [&](int i) { return make_float2(tot[2 * i], tot[2 * i + 1]); }, [&](int g, float2 v) {
+        const float d = v.x / N;
+        out[g] = make_float2(gs[g] + d, v.y - v.x * d);
+    });
 }
 
-// grid (runs of rows, batch), walked from the end
-template <typename T, bool PER>
-__global__ __launch_bounds__(1024) void gn_apply_kernel(const GnArgs a, int run_rows) {
-    constexpr int V = NormElem<T>::V, NG = PER ? V : 1;
+// grid (runs of rows, batch), walked from the end.  A thread's first rows are on their way while the chunks' statistics are merged.
+template <typename T, int M, bool SILU>
+__global__ __launch_bounds__(1024, 6) void gn_apply_kernel(const GnArgs a, int run_rows) {
+    constexpr int V = NormElem<T>::V, NG = M ? V : 1, U = 4;
     extern __shared__ float lds[];
     const NormShape& s = a.s;
     const int t = threadIdx.x, TB = blockDim.x, cols = s.cols;
     const int b = s.batch - 1 - blockIdx.y, run = gridDim.x - 1 - blockIdx.x;
-    const int RT = TB / cols, r = t / cols, j = t - r * cols;
+    const int RT = (int)fdiv((unsigned)TB, s.by_cols), r = (int)fdiv((unsigned)t, s.by_cols), j = t - r * cols;
     float *red = lds, *gmean = red + 2 * TB, *grstd = gmean + s.groups;
+    Column<T, M> col;
+    col.init(s, j);
+    const int row0 = run * run_rows + r;
+    const int row1 = r < RT ? (run * run_rows + run_rows < s.vrows ? run * run_rows + run_rows : s.vrows) : 0;
+    const T* xb = static_cast<const T*>(a.x) + (size_t)b * a.x_img + col.off;
+    T* yb = static_cast<T*>(a.y) + (size_t)b * a.y_img + col.off;
+    Raw v[U];
+    auto load = [&](int row) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (row + u * RT < row1) v[u] = ld_col<T, M>(xb + (size_t)(row + u * RT) * a.x_row, col.valid(s, row + u * RT));
+    };
+    load(row0);
+    float mean[NG], A[V], B[V];
+    col.params(s, a.weight, 1.f, A);
+    col.params(s, a.bias, 0.f, B);
     norm_merge_chunks(s, a.part, b, red, gmean, grstd);
     if (a.mean && run == 0) {
         for (int g = t; g < s.groups; g += TB) {
@@ -331,49 +396,27 @@ __global__ __launch_bounds__(1024) void gn_apply_kernel(const GnArgs a, int run_
             a.rstd[(size_t)b * s.groups + g] = grstd[g];
         }
     }
-    if (r >= RT) return;
-    Column<T, PER> col;
-    col.init(s, j);
-    float mean[NG], A[V], B[V];
 #pragma unroll
     for (int e = 0; e < NG; ++e) mean[e] = gmean[col.grp[e]];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-        const int c = col.channel(s, e);
-        A[e] = ld_param(a.weight, c, s.param_dtype, 1.f) * grstd[col.grp[PER ? e : 0]];
-        B[e] = ld_param(a.bias, c, s.param_dtype, 0.f);
-    }
-    const int row0 = run * run_rows;
-    const int row1 = row0 + run_rows < s.vrows ? row0 + run_rows : s.vrows;
-    const T* xb = static_cast<const T*>(a.x) + (size_t)b * a.x_img + col.off;
-    T* yb = static_cast<T*>(a.y) + (size_t)b * a.y_img + col.off;
-    int row = row0 + r;
-    for (; row + 3 * RT < row1 - (PER ? 1 : 0); row += 4 * RT) {
-        T v[4][V], o[V];
+    for (int e = 0; e < V; ++e) A[e] *= grstd[col.grp[M ? e : 0]];
+    for (int row = row0; row < row1; row += U * RT) {
+        Raw o[U];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) ld_vec(xb + (size_t)(row + u * RT) * a.x_row, v[u]);
+        for (int u = 0; u < U; ++u) o[u] = normalise<T, SILU, NG>(v[u], mean, A, B, s.slope);
+        load(row + U * RT);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            normalise<T, NG>(v[u], o, mean, A, B, s.act, s.slope);
-            st_vec(yb + (size_t)(row + u * RT) * a.y_row, o);
-        }
-    }
-    for (; row < row1; row += RT) {
-        const int nv = col.valid(s, row);
-        if (!nv) continue;
-        T v[V], o[V];
-        ld_col<T, PER>(xb + (size_t)row * a.x_row, nv, v);
-        normalise<T, NG>(v, o, mean, A, B, s.act, s.slope);
-        st_col<T, PER>(yb + (size_t)row * a.y_row, nv, o);
+        for (int u = 0; u < U; ++u)
+            if (row + u * RT < row1) st_col<T, M>(yb + (size_t)(row + u * RT) * a.y_row, col.valid(s, row + u * RT), o[u]);
     }
 }
 
 // ------------------------------------------------------------------------------------------ backward
 
 // Parameters of a thread's column for the gradient: mean, rstd of its groups, gamma and beta of its channels
-template <typename T, bool PER>
-struct GradColumn : Column<T, PER> {
-    static constexpr int V = NormElem<T>::V, NG = PER ? V : 1;
+template <typename T, int M>
+struct GradColumn : Column<T, M> {
+    static constexpr int V = NormElem<T>::V, NG = M ? V : 1;
     float mean[NG], rstd[NG], gamma[V], beta[V];
     __device__ __forceinline__ void load(const GnArgs& a, int b, int col) {
         const NormShape& s = a.s;
@@ -383,34 +426,34 @@ struct GradColumn : Column<T, PER> {
             mean[e] = a.mean[(size_t)b * s.groups + this->grp[e]];
             rstd[e] = a.rstd[(size_t)b * s.groups + this->grp[e]];
         }
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const int c = this->channel(s, e);
-            gamma[e] = ld_param(a.weight, c, s.param_dtype, 1.f);
-            beta[e] = ld_param(a.bias, c, s.param_dtype, 0.f);
-        }
+        this->params(s, a.weight, 1.f, gamma);
+        this->params(s, a.bias, 0.f, beta);
     }
     // xh and dz of one vector
-    __device__ __forceinline__ void local(const T (&x)[V], const T (&dy)[V], float (&xh)[V], float (&dz)[V], int act, float slope) const {
+    template <bool SILU>
+    __device__ __forceinline__ void local(Raw& rx, Raw& rd, float (&xh)[V], float (&dz)[V], float slope) const {
+        const NormArr<T> x = unpack<T>(rx), dy = unpack<T>(rd);
         float z[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            xh[e] = ((float)x[e] - mean[PER ? e : 0]) * rstd[PER ? e : 0];
+            xh[e] = ((float)x.v[e] - mean[M ? e : 0]) * rstd[M ? e : 0];
             z[e] = __builtin_fmaf(xh[e], gamma[e], beta[e]);
-            dz[e] = (float)dy[e];
+            dz[e] = (float)dy.v[e];
         }
-        norm_act_grad(dz, z, act, slope);
+        norm_act_grad<SILU>(dz, z, slope);
     }
     // dx of one vector from s1 = S1 / n and s2 = S2 / n of its groups
-    __device__ __forceinline__ void grad(const float (&xh)[V], const float (&dz)[V], const float (&s1)[NG], const float (&s2)[NG], T (&dx)[V]) const {
+    __device__ __forceinline__ Raw grad(const float (&xh)[V], const float (&dz)[V], const float (&s1)[NG], const float (&s2)[NG]) const {
 #pragma clang fp contract(off)  // a group of one value has gamma dz = S1 exactly and a gradient of exactly zero
+        NormArr<T> dx;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             const float w = gamma[e] * dz[e];
-            const float u = w - s1[PER ? e : 0];
-            const float v = xh[e] * s2[PER ? e : 0];
-            dx[e] = (T)(rstd[PER ? e : 0] * (u - v));
+            const float u = w - s1[M ? e : 0];
+            const float v = xh[e] * s2[M ? e : 0];
+            dx.v[e] = (T)(rstd[M ? e : 0] * (u - v));
         }
+        return __builtin_bit_cast(Raw, dx);
     }
 };
 
@@ -426,34 +469,40 @@ __device__ __forceinline__ void grad_sums(const GnArgs& a, const float* tot, int
         for (int k = 0; k < s.k; ++k) v += at(k * s.c + c, which);
         out[(size_t)which * s.c + c0 + c] = v;
     }
-    for (int which = 0; which < 2; ++which)
-        group_sum(G, s.cpg, s.k, s.c, [&](int i) { return ld_param(a.weight, c0 + i % s.c, s.param_dtype, 1.f) * at(i, which); },
-                  [&](int g, float v) { gs[2 * g + which] = v * scale; });
+    group_sum2(G, s.cpg, s.k, s.c,
+               [&](int i) {
+                   const float w = ld_param(a.weight, c0 + i - (int)fdiv((unsigned)i, s.by_c) * s.c, s.param_dtype, 1.f);
+                   return make_float2(w * at(i, 0), w * at(i, 1));
+               },
+               [&](int g, float2 v) {
+                   gs[2 * g] = v.x * scale;
+                   gs[2 * g + 1] = v.y * scale;
+               });
 }
 
-// grid (slices, batch); LDS: part[blockDim.x * 2 V], tot[cols * 2 V], gs[2 * groups of the slice]
-template <typename T, bool PER, int R>
-__global__ __launch_bounds__(R > 4 ? 512 : 256) void gn_bwd_resident_kernel(const GnArgs a, int cols) {
-    constexpr int V = NormElem<T>::V, NG = PER ? V : 1;
+// grid: slices * batch; LDS: part[blockDim.x * 2 V], tot[cols * 2 V], gs[2 * groups of the slice]
+template <typename T, int M, bool SILU, int R>
+__global__ __launch_bounds__(R > 4 ? 512 : 256, R > 4 && sizeof(T) == 2 ? 3 : 4) void gn_bwd_resident_kernel(const GnArgs a, const FastDiv by_cols, int slices) {
+    constexpr int V = NormElem<T>::V, NG = M ? V : 1;
     extern __shared__ float lds[];
     const NormShape& s = a.s;
-    const int t = threadIdx.x, TB = blockDim.x, b = blockIdx.y;
-    const int RT = TB / cols, r = t / cols, j = t - r * cols;
+    // slices of an image share cache lines: neighbours run on one XCD, behind one L2
+    const int at = xcd_remap(blockIdx.x, gridDim.x), b = at / slices, slice = at - b * slices;
+    const int t = threadIdx.x, TB = blockDim.x, cols = (int)by_cols.d;
+    const int RT = (int)fdiv((unsigned)TB, by_cols), r = (int)fdiv((unsigned)t, by_cols), j = t - r * cols;
     const bool active = r < RT;
     float *part = lds, *tot = part + TB * 2 * V, *gs = tot + cols * 2 * V;
-    GradColumn<T, PER> col;
-    col.load(a, b, blockIdx.x * cols + j);
+    GradColumn<T, M> col;
+    col.load(a, b, slice * cols + j);
     const T* xb = static_cast<const T*>(a.x) + (size_t)b * a.x_img + col.off;
     const T* db = static_cast<const T*>(a.dy) + (size_t)b * a.dy_img + col.off;
-    T rx[R][V], rd[R][V];
-    int nv[R];
+    Raw rx[R], rd[R];
+    auto valid = [&](int i) { return active && r + i * RT < s.vrows ? col.valid(s, r + i * RT) : 0; };
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        const int row = r + i * RT;
-        nv[i] = active && row < s.vrows ? col.valid(s, row) : 0;
-        if (nv[i]) {
-            ld_col<T, PER>(xb + (size_t)row * a.x_row, nv[i], rx[i]);
-            ld_col<T, PER>(db + (size_t)row * a.dy_row, nv[i], rd[i]);
+        if (const int nv = valid(i)) {
+            rx[i] = ld_col<T, M>(xb + (size_t)(r + i * RT) * a.x_row, nv);
+            rd[i] = ld_col<T, M>(db + (size_t)(r + i * RT) * a.dy_row, nv);
         }
     }
     float acc[2 * V];
@@ -461,19 +510,19 @@ __global__ __launch_bounds__(R > 4 ? 512 : 256) void gn_bwd_resident_kernel(cons
     for (int e = 0; e < 2 * V; ++e) acc[e] = 0.f;
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (nv[i]) {
+        if (const int nv = valid(i)) {
             float xh[V], dz[V];
-            col.local(rx[i], rd[i], xh, dz, s.act, s.slope);
+            col.template local<SILU>(rx[i], rd[i], xh, dz, s.slope);
 #pragma unroll
             for (int e = 0; e < V; ++e)
-                if (!PER || e < nv[i]) {
+                if (M != kCut || e < nv) {
                     acc[e] += dz[e];
                     acc[V + e] = __builtin_fmaf(dz[e], xh[e], acc[V + e]);
                 }
         }
     col_sum<2 * V>(acc, j, r, RT, cols, part, tot);
-    const int c0 = s.k > 1 ? 0 : blockIdx.x * cols * V, channels = s.k > 1 ? s.c : cols * V;
-    const int g0 = c0 / s.cpg, G = channels / s.cpg;
+    const int c0 = s.k > 1 ? 0 : slice * cols * V, channels = s.k > 1 ? s.c : cols * V;
+    const int g0 = (int)fdiv(c0, s.by_cpg), G = (int)fdiv(channels, s.by_cpg);
     grad_sums<V>(a, tot, c0, channels, G, 1.f / ((float)s.pixels * (float)s.cpg), a.cpart + (size_t)b * 2 * s.c, gs);
     if (!active || !a.dx) return;
     float s1[NG], s2[NG];
@@ -485,25 +534,23 @@ __global__ __launch_bounds__(R > 4 ? 512 : 256) void gn_bwd_resident_kernel(cons
     T* ob = static_cast<T*>(a.dx) + (size_t)b * a.dx_img + col.off;
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (nv[i]) {
+        if (const int nv = valid(i)) {
             float xh[V], dz[V];
-            T dx[V];
-            col.local(rx[i], rd[i], xh, dz, s.act, s.slope);
-            col.grad(xh, dz, s1, s2, dx);
-            st_col<T, PER>(ob + (size_t)(r + i * RT) * a.dx_row, nv[i], dx);
+            col.template local<SILU>(rx[i], rd[i], xh, dz, s.slope);
+            st_col<T, M>(ob + (size_t)(r + i * RT) * a.dx_row, nv, col.grad(xh, dz, s1, s2));
         }
 }
 
 // grid (chunks, batch); LDS as above for all groups
-template <typename T, bool PER>
-__global__ __launch_bounds__(1024) void gn_bwd_stats_kernel(const GnArgs a) {
+template <typename T, int M, bool SILU>
+__global__ __launch_bounds__(1024, M == kUniform || sizeof(T) == 4 ? 5 : 4) void gn_bwd_stats_kernel(const GnArgs a) {
     constexpr int V = NormElem<T>::V;
     extern __shared__ float lds[];
     const NormShape& s = a.s;
     const int t = threadIdx.x, TB = blockDim.x, b = blockIdx.y, cols = s.cols;
-    const int RT = TB / cols, r = t / cols, j = t - r * cols;
+    const int RT = (int)fdiv((unsigned)TB, s.by_cols), r = (int)fdiv((unsigned)t, s.by_cols), j = t - r * cols;
     float *part = lds, *tot = part + TB * 2 * V, *gs = tot + cols * 2 * V;
-    GradColumn<T, PER> col;
+    GradColumn<T, M> col;
     col.load(a, b, j);
     float acc[2 * V];
 #pragma unroll
@@ -513,32 +560,30 @@ __global__ __launch_bounds__(1024) void gn_bwd_stats_kernel(const GnArgs a) {
     if (r < RT) {
         const T* xb = static_cast<const T*>(a.x) + (size_t)b * a.x_img + col.off;
         const T* db = static_cast<const T*>(a.dy) + (size_t)b * a.dy_img + col.off;
-        auto take = [&](const T (&x)[V], const T (&d)[V], int nv) {
+        auto take = [&](Raw& x, Raw& d, int nv) {
             float xh[V], dz[V];
-            col.local(x, d, xh, dz, s.act, s.slope);
+            col.template local<SILU>(x, d, xh, dz, s.slope);
 #pragma unroll
             for (int e = 0; e < V; ++e)
-                if (!PER || e < nv) {
+                if (M != kCut || e < nv) {
                     acc[e] += dz[e];
                     acc[V + e] = __builtin_fmaf(dz[e], xh[e], acc[V + e]);
                 }
         };
         int row = row0 + r;
-        for (; row + RT < row1 - (PER ? 1 : 0); row += 2 * RT) {
-            T x[2][V], d[2][V];
+        for (; row + RT < row1 - (M == kCut ? 1 : 0); row += 2 * RT) {
+            Raw x[2], d[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                ld_vec(xb + (size_t)(row + u * RT) * a.x_row, x[u]);
-                ld_vec(db + (size_t)(row + u * RT) * a.dy_row, d[u]);
+                x[u] = ld_col<T, M>(xb + (size_t)(row + u * RT) * a.x_row, V);
+                d[u] = ld_col<T, M>(db + (size_t)(row + u * RT) * a.dy_row, V);
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) take(x[u], d[u], V);
         }
         for (; row < row1; row += RT) {
             const int nv = col.valid(s, row);
-            T x[V], d[V];
-            ld_col<T, PER>(xb + (size_t)row * a.x_row, nv, x);
-            ld_col<T, PER>(db + (size_t)row * a.dy_row, nv, d);
+            Raw x = ld_col<T, M>(xb + (size_t)row * a.x_row, nv), d = ld_col<T, M>(db + (size_t)row * a.dy_row, nv);
             take(x, d, nv);
         }
     }
@@ -548,16 +593,65 @@ __global__ __launch_bounds__(1024) void gn_bwd_stats_kernel(const GnArgs a) {
     for (int g = t; g < s.groups; g += TB) a.part[at * s.groups + g] = make_float2(gs[2 * g], gs[2 * g + 1]);
 }
 
-// grid (runs of rows, batch), walked from the end; LDS: red[2 * blockDim.x], gs[2 * groups]
-template <typename T, bool PER>
-__global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(const GnArgs a, int run_rows) {
-    constexpr int V = NormElem<T>::V, NG = PER ? V : 1;
+// dbeta_c and dgamma_c: the rows of cpart ([rows][2][c]) added up, 16 of the 2 c columns by T threads.  red: T floats of LDS.
+__device__ __forceinline__ void sum_params(const float* __restrict__ cpart, int rows, int c, int dt, void* dweight, void* dbias, int block, float* red) {
+    const int T = blockDim.x / 16 * 16, t = threadIdx.x;
+    const int lc = t & 15, q = t >> 4, Q = T >> 4;
+    const int i = block * 16 + lc;
+    float v = 0.f;
+    if (t < T && i < 2 * c) {
+#pragma unroll 8
+        for (int k = q; k < rows; k += Q) v += cpart[(size_t)k * 2 * c + i];
+    }
+    if (t < T) red[q * 16 + lc] = v;
+    __syncthreads();
+    if (q || i >= 2 * c) return;
+    for (int k = 1; k < Q; ++k) v += red[k * 16 + lc];
+    if (i < c) {
+        if (dbias) st_param(dbias, i, dt, v);
+    } else if (dweight) {
+        st_param(dweight, i - c, dt, v);
+    }
+}
+__global__ __launch_bounds__(256) void gn_dparam_kernel(const float* __restrict__ cpart, int rows, int c, int dt, void* dweight, void* dbias) {
+    __shared__ float red[256];
+    sum_params(cpart, rows, c, dt, dweight, dbias, blockIdx.x, red);
+}
+
+// grid (param_blocks + runs of rows * batch): the first workgroups add up the parameters' gradients, beside the others' work on dx, which
+// walk the images from the end.  LDS: red[2 * blockDim.x], gs[2 * groups]
+template <typename T, int M, bool SILU>
+__global__ __launch_bounds__(1024, M == kUniform || sizeof(T) == 4 ? 5 : 4) void gn_bwd_apply_kernel(const GnArgs a, int run_rows, int runs, int param_blocks) {
+    constexpr int V = NormElem<T>::V, NG = M ? V : 1, U = 2;
     extern __shared__ float lds[];
     const NormShape& s = a.s;
     const int t = threadIdx.x, TB = blockDim.x, cols = s.cols;
-    const int b = s.batch - 1 - blockIdx.y, run = gridDim.x - 1 - blockIdx.x;
-    const int RT = TB / cols, r = t / cols, j = t - r * cols;
     float *red = lds, *gs = lds + 2 * TB;
+    if ((int)blockIdx.x < param_blocks) {
+        sum_params(a.cpart, s.batch * s.chunks, s.c, s.param_dtype, a.dweight, a.dbias, blockIdx.x, red);
+        return;
+    }
+    const int at = gridDim.x - 1 - blockIdx.x;
+    const int b = at / runs, run = at - b * runs;
+    const int RT = (int)fdiv((unsigned)TB, s.by_cols), r = (int)fdiv((unsigned)t, s.by_cols), j = t - r * cols;
+    GradColumn<T, M> col;
+    col.load(a, b, j);
+    const T* xb = static_cast<const T*>(a.x) + (size_t)b * a.x_img + col.off;
+    const T* db = static_cast<const T*>(a.dy) + (size_t)b * a.dy_img + col.off;
+    T* ob = static_cast<T*>(a.dx) + (size_t)b * a.dx_img + col.off;
+    const int row0 = run * run_rows + r;
+    const int row1 = r < RT ? (run * run_rows + run_rows < s.vrows ? run * run_rows + run_rows : s.vrows) : 0;
+    Raw x[U], d[U];
+    auto load = [&](int row) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (row + u * RT < row1) {
+                const int nv = col.valid(s, row + u * RT);
+                x[u] = ld_col<T, M>(xb + (size_t)(row + u * RT) * a.x_row, nv);
+                d[u] = ld_col<T, M>(db + (size_t)(row + u * RT) * a.dy_row, nv);
+            }
+    };
+    load(row0);
     const float2* pb = a.part + (size_t)b * s.chunks * s.groups;
     for (int g0 = 0; g0 < s.groups; g0 += TB) {  // S1 / n and S2 / n of every group: the chunks' sums added up
         const int G = s.groups - g0 < TB ? s.groups - g0 : TB;
@@ -584,68 +678,24 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(const GnArgs a, int 
         }
         __syncthreads();
     }
-    if (r >= RT) return;
-    GradColumn<T, PER> col;
-    col.load(a, b, j);
     float s1[NG], s2[NG];
 #pragma unroll
     for (int e = 0; e < NG; ++e) {
         s1[e] = gs[2 * col.grp[e]];
         s2[e] = gs[2 * col.grp[e] + 1];
     }
-    const int row0 = run * run_rows;
-    const int row1 = row0 + run_rows < s.vrows ? row0 + run_rows : s.vrows;
-    const T* xb = static_cast<const T*>(a.x) + (size_t)b * a.x_img + col.off;
-    const T* db = static_cast<const T*>(a.dy) + (size_t)b * a.dy_img + col.off;
-    T* ob = static_cast<T*>(a.dx) + (size_t)b * a.dx_img + col.off;
-    int row = row0 + r;
-    for (; row + RT < row1 - (PER ? 1 : 0); row += 2 * RT) {
-        T x[2][V], d[2][V], o[V];
+    for (int row = row0; row < row1; row += U * RT) {
+        Raw o[U];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            ld_vec(xb + (size_t)(row + u * RT) * a.x_row, x[u]);
-            ld_vec(db + (size_t)(row + u * RT) * a.dy_row, d[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < U; ++u) {
             float xh[V], dz[V];
-            col.local(x[u], d[u], xh, dz, s.act, s.slope);
-            col.grad(xh, dz, s1, s2, o);
-            st_vec(ob + (size_t)(row + u * RT) * a.dx_row, o);
+            col.template local<SILU>(x[u], d[u], xh, dz, s.slope);
+            o[u] = col.grad(xh, dz, s1, s2);
         }
-    }
-    for (; row < row1; row += RT) {
-        const int nv = col.valid(s, row);
-        if (!nv) continue;
-        T x[V], d[V], o[V];
-        ld_col<T, PER>(xb + (size_t)row * a.x_row, nv, x);
-        ld_col<T, PER>(db + (size_t)row * a.dy_row, nv, d);
-        float xh[V], dz[V];
-        col.local(x, d, xh, dz, s.act, s.slope);
-        col.grad(xh, dz, s1, s2, o);
-        st_col<T, PER>(ob + (size_t)row * a.dx_row, nv, o);
-    }
-}
-
-// dbeta_c and dgamma_c: the rows of cpart ([rows][2][c]) added up.  A workgroup takes 16 of the 2 c columns, 16 threads each.
-__global__ __launch_bounds__(256) void gn_dparam_kernel(const float* __restrict__ cpart, int rows, int c, int dt, void* dweight, void* dbias) {
-    __shared__ float red[16][17];
-    const int lc = threadIdx.x & 15, q = threadIdx.x >> 4;
-    const int i = blockIdx.x * 16 + lc;
-    float v = 0.f;
-    if (i < 2 * c) {
-#pragma unroll 8
-        for (int k = q; k < rows; k += 16) v += cpart[(size_t)k * 2 * c + i];
-    }
-    red[q][lc] = v;
-    __syncthreads();
-    if (q || i >= 2 * c) return;
+        load(row + U * RT);
 #pragma unroll
-    for (int k = 1; k < 16; ++k) v += red[k][lc];
-    if (i < c) {
-        if (dbias) st_param(dbias, i, dt, v);
-    } else if (dweight) {
-        st_param(dweight, i - c, dt, v);
+        for (int u = 0; u < U; ++u)
+            if (row + u * RT < row1) st_col<T, M>(ob + (size_t)(row + u * RT) * a.dx_row, col.valid(s, row + u * RT), o[u]);
     }
 }
 
@@ -657,14 +707,16 @@ int split_threads(int cols) {
     return (rows * cols + 63) / 64 * 64;
 }
 
-// Rows of a workgroup of the second pass: 32 KiB
+// Virtual rows of a workgroup of the second pass
 int run_rows(const NormShape& s, int esize) {
-    const long long rows = (32 << 10) / ((long long)s.W * esize);
+    const long long rows = norm_run_bytes(s, esize) / ((long long)s.W * esize);
     return rows < 1 ? 1 : (int)rows;
 }
 
-// A resident slice: the fewest columns that hold whole groups and 64 bytes of a pixel (half a cache line; narrower slices
-// read lines that other workgroups read again).  False where no slice fits R vectors a thread.
+constexpr int kResidentAlone = 32 << 10;  // bytes of a slice that few workgroups may hold all the same
+
+// A resident slice: whole groups, and 64 bytes of a pixel (half a cache line, so that little is read twice) where that leaves a workgroup
+// for every compute unit.  False where no slice fits the registers, or where a few workgroups would work long while the chip idles.
 struct Resident {
     int cols, threads, r;
 };
@@ -672,10 +724,11 @@ bool resident_of(const NormShape& s, int esize, const int (&cap)[3][2], Resident
     const int V = 16 / esize;
     int cols = s.cols;
     if (s.k == 1) {
-        const int unit = s.cpg / norm_gcd(s.cpg, V);  // lcm(cpg, V) / V columns hold whole groups and whole vectors
-        cols = unit;
-        while (cols * 16 < 64 && cols * 2 <= s.cols && s.cols % (cols * 2) == 0) cols *= 2;
+        cols = s.cpg / norm_gcd(s.cpg, V);  // lcm(cpg, V) / V columns hold whole groups and whole vectors
+        while (cols * 16 < 64 && s.cols % (cols * 2) == 0 && (long long)s.batch * (s.cols / (cols * 2)) >= 256) cols *= 2;
     }
+    const long long wgs = (long long)s.batch * (s.cols / cols), bytes = (long long)s.vrows * cols * 16;
+    if (bytes > kResidentAlone && wgs < 128) return false;
     for (const auto& c : cap) {
         const int threads = c[0], r = c[1];
         if (cols > threads) continue;
@@ -698,6 +751,8 @@ GnArgs make_args(const y5_group_norm_desc& d, const NormShape& s) {
     a.bias = d.bias;
     a.y = d.y;
     a.dx = d.dx;
+    a.dweight = d.dweight;
+    a.dbias = d.dbias;
     a.mean = d.mean;
     a.rstd = d.rstd;
     const int ld[4] = {d.x_ld, d.y_ld, d.dy_ld, d.dx_ld};
@@ -724,55 +779,71 @@ int with_lds(F kernel, size_t bytes) {  // more than 64 KiB of LDS have to be as
         Y5_LAUNCH_CHECK(NAME);                                                              \
     } while (0)
 
-template <typename T, bool PER>
+template <typename T, int M>
 int stats(const GnArgs& a, hipStream_t st) {
     const int threads = split_threads(a.s.cols);
-    const size_t lds = ((size_t)(threads + a.s.cols) * (PER ? NormElem<T>::V : 1) + a.s.groups) * 4;
-    GN_LAUNCH("gn_stats_kernel", (gn_stats_kernel<T, PER>), dim3(a.s.chunks, a.s.batch), threads, lds, a);
+    const size_t lds = ((size_t)(threads + a.s.cols) * 2 * (M ? NormElem<T>::V : 1) + a.s.groups) * 4;
+    GN_LAUNCH("gn_stats_kernel", (gn_stats_kernel<T, M>), dim3(a.s.chunks, a.s.batch), threads, lds, a);
     return Y5_OK;
 }
 
-template <typename T, bool PER>
+template <typename T, int M, bool SILU>
 int forward(const GnArgs& a, const Resident* res, hipStream_t st) {
     const NormShape& s = a.s;
-    constexpr int V = NormElem<T>::V, NG = PER ? V : 1;
+    constexpr int V = NormElem<T>::V, NG = M ? V : 1;
     if (res) {
-        const dim3 grid(s.k == 1 ? s.cols / res->cols : 1, s.batch);
+        const int slices = s.k == 1 ? s.cols / res->cols : 1;
+        const dim3 grid((unsigned)slices * s.batch);
         const size_t lds = ((size_t)(res->threads + res->cols) * NG + 2 * (s.k == 1 ? res->cols * V / s.cpg : s.groups)) * 4;
-        if (res->r == 4) GN_LAUNCH("gn_resident_kernel", (gn_resident_kernel<T, PER, 4>), grid, res->threads, lds, a, res->cols);
-        else if (res->r == 8) GN_LAUNCH("gn_resident_kernel", (gn_resident_kernel<T, PER, 8>), grid, res->threads, lds, a, res->cols);
-        else GN_LAUNCH("gn_resident_kernel", (gn_resident_kernel<T, PER, 16>), grid, res->threads, lds, a, res->cols);
+        if (res->r == 4) GN_LAUNCH("gn_resident_kernel", (gn_resident_kernel<T, M, SILU, 4>), grid, res->threads, lds, a, make_fastdiv((unsigned)res->cols), slices);
+        else if (res->r == 8) GN_LAUNCH("gn_resident_kernel", (gn_resident_kernel<T, M, SILU, 8>), grid, res->threads, lds, a, make_fastdiv((unsigned)res->cols), slices);
+        else GN_LAUNCH("gn_resident_kernel", (gn_resident_kernel<T, M, SILU, 16>), grid, res->threads, lds, a, make_fastdiv((unsigned)res->cols), slices);
         return Y5_OK;
     }
-    if (int rc = stats<T, PER>(a, st)) return rc;
+    if (int rc = stats<T, M>(a, st)) return rc;
     const int threads = split_threads(s.cols), rr = run_rows(s, sizeof(T));
     const size_t lds = (2 * (size_t)threads + 2 * s.groups) * 4;
-    GN_LAUNCH("gn_apply_kernel", (gn_apply_kernel<T, PER>), dim3((s.vrows + rr - 1) / rr, s.batch), threads, lds, a, rr);
+    GN_LAUNCH("gn_apply_kernel", (gn_apply_kernel<T, M, SILU>), dim3((s.vrows + rr - 1) / rr, s.batch), threads, lds, a, rr);
     return Y5_OK;
 }
 
-template <typename T, bool PER>
-int backward(const GnArgs& a, const Resident* res, void* dweight, void* dbias, hipStream_t st) {
+template <typename T, int M, bool SILU>
+int backward(const GnArgs& a, const Resident* res, hipStream_t st) {
     const NormShape& s = a.s;
     constexpr int V = NormElem<T>::V;
     if (res) {
-        const dim3 grid(s.k == 1 ? s.cols / res->cols : 1, s.batch);
+        const int slices = s.k == 1 ? s.cols / res->cols : 1;
+        const dim3 grid((unsigned)slices * s.batch);
         const size_t lds = ((size_t)(res->threads + res->cols) * 2 * V + 2 * (s.k == 1 ? res->cols * V / s.cpg : s.groups)) * 4;
-        if (res->r == 2) GN_LAUNCH("gn_bwd_resident_kernel", (gn_bwd_resident_kernel<T, PER, 2>), grid, res->threads, lds, a, res->cols);
-        else if (res->r == 4) GN_LAUNCH("gn_bwd_resident_kernel", (gn_bwd_resident_kernel<T, PER, 4>), grid, res->threads, lds, a, res->cols);
-        else GN_LAUNCH("gn_bwd_resident_kernel", (gn_bwd_resident_kernel<T, PER, 8>), grid, res->threads, lds, a, res->cols);
+        if (res->r == 2) GN_LAUNCH("gn_bwd_resident_kernel", (gn_bwd_resident_kernel<T, M, SILU, 2>), grid, res->threads, lds, a, make_fastdiv((unsigned)res->cols), slices);
+        else if (res->r == 4) GN_LAUNCH("gn_bwd_resident_kernel", (gn_bwd_resident_kernel<T, M, SILU, 4>), grid, res->threads, lds, a, make_fastdiv((unsigned)res->cols), slices);
+        else GN_LAUNCH("gn_bwd_resident_kernel", (gn_bwd_resident_kernel<T, M, SILU, 8>), grid, res->threads, lds, a, make_fastdiv((unsigned)res->cols), slices);
     } else {
-        const int threads = split_threads(s.cols), rr = run_rows(s, sizeof(T));
+        const int threads = split_threads(s.cols), rr = run_rows(s, sizeof(T)), runs = (s.vrows + rr - 1) / rr;
         size_t lds = ((size_t)(threads + s.cols) * 2 * V + 2 * s.groups) * 4;
-        GN_LAUNCH("gn_bwd_stats_kernel", (gn_bwd_stats_kernel<T, PER>), dim3(s.chunks, s.batch), threads, lds, a);
-        lds = (2 * (size_t)threads + 2 * s.groups) * 4;
-        if (a.dx) GN_LAUNCH("gn_bwd_apply_kernel", (gn_bwd_apply_kernel<T, PER>), dim3((s.vrows + rr - 1) / rr, s.batch), threads, lds, a, rr);
+        GN_LAUNCH("gn_bwd_stats_kernel", (gn_bwd_stats_kernel<T, M, SILU>), dim3(s.chunks, s.batch), threads, lds, a);
+        if (a.dx) {
+            const int param_blocks = a.dweight || a.dbias ? (2 * s.c + 15) / 16 : 0;
+            Y5_REQUIRE((long long)runs * s.batch + param_blocks <= 0x7fffffffLL, "group_norm_backward: %d images of %d pixels", s.batch, s.pixels);
+            lds = (2 * (size_t)threads + 2 * s.groups) * 4;
+            GN_LAUNCH("gn_bwd_apply_kernel", (gn_bwd_apply_kernel<T, M, SILU>), dim3(runs * s.batch + param_blocks), threads, lds, a, rr, runs, param_blocks);
+            return Y5_OK;
+        }
     }
-    if (dweight || dbias) {
+    if (a.dweight || a.dbias) {
         const int rows = res ? s.batch : s.batch * s.chunks;
-        GN_LAUNCH("gn_dparam_kernel", gn_dparam_kernel, dim3((2 * s.c + 15) / 16), 256, 0, a.cpart, rows, s.c, s.param_dtype, dweight, dbias);
+        GN_LAUNCH("gn_dparam_kernel", gn_dparam_kernel, dim3((2 * s.c + 15) / 16), 256, 0, a.cpart, rows, s.c, s.param_dtype, a.dweight, a.dbias);
     }
     return Y5_OK;
+}
+
+template <typename T, int M>
+int forward_act(const GnArgs& a, const Resident* res, hipStream_t st) {
+    return a.s.act == Y5_ACT_SILU ? forward<T, M, true>(a, res, st) : forward<T, M, false>(a, res, st);
+}
+template <typename T, int M>
+int backward_act(const GnArgs& a, const Resident* res, hipStream_t st) {
+    return a.s.act == Y5_ACT_SILU ? backward<T, M, true>(a, res, st) : backward<T, M, false>(a, res, st);
 }
 
 struct GnWork {
@@ -785,7 +856,13 @@ GnWork work_of(const NormShape& s, bool resident, bool bwd) {
     return w;
 }
 
-bool per_element(const NormShape& s, int esize) { return s.k > 1 || s.cpg % (16 / esize) != 0; }
+int mode_of(const NormShape& s, int esize) { return s.k > 1 ? kCut : s.cpg % (16 / esize) != 0 ? kMixed : kUniform; }
+
+// f<type, mode>(args...) of a call's dtype and mode
+#define GN_DISPATCH(F, DTYPE, MODE, ...)                                                                                              \
+    ((DTYPE) == Y5_F16    ? ((MODE) == kCut ? F<f16, kCut>(__VA_ARGS__) : (MODE) == kMixed ? F<f16, kMixed>(__VA_ARGS__) : F<f16, kUniform>(__VA_ARGS__)) \
+     : (DTYPE) == Y5_BF16 ? ((MODE) == kCut ? F<bf16, kCut>(__VA_ARGS__) : (MODE) == kMixed ? F<bf16, kMixed>(__VA_ARGS__) : F<bf16, kUniform>(__VA_ARGS__)) \
+                          : ((MODE) == kCut ? F<float, kCut>(__VA_ARGS__) : (MODE) == kMixed ? F<float, kMixed>(__VA_ARGS__) : F<float, kUniform>(__VA_ARGS__)))
 
 }  // namespace
 
@@ -794,10 +871,7 @@ int y5_launch_group_norm_stats(const y5_group_norm_desc& d, hipStream_t st) {
     if (int rc = norm_make_shape(d, &s)) return rc;
     GnArgs a = make_args(d, s);
     a.part = static_cast<float2*>(d.workspace);
-    const bool per = per_element(s, norm_elem_size(d.dtype));
-    if (d.dtype == Y5_F16) return per ? stats<f16, true>(a, st) : stats<f16, false>(a, st);
-    if (d.dtype == Y5_BF16) return per ? stats<bf16, true>(a, st) : stats<bf16, false>(a, st);
-    return per ? stats<float, true>(a, st) : stats<float, false>(a, st);
+    return GN_DISPATCH(stats, d.dtype, mode_of(s, norm_elem_size(d.dtype)), a, st);
 }
 
 int y5_group_norm_work(const y5_group_norm_desc& d, int what, size_t* bytes) {
@@ -826,11 +900,7 @@ int y5_launch_group_norm(const y5_group_norm_desc& d, hipStream_t st) {
     Y5_REQUIRE(!w.total || y5_aligned16(d.workspace), "group_norm: misaligned workspace");
     GnArgs a = make_args(d, s);
     a.part = static_cast<float2*>(d.workspace);
-    const bool per = per_element(s, es);
-    const Resident* rp = res ? &r : nullptr;
-    if (d.dtype == Y5_F16) return per ? forward<f16, true>(a, rp, st) : forward<f16, false>(a, rp, st);
-    if (d.dtype == Y5_BF16) return per ? forward<bf16, true>(a, rp, st) : forward<bf16, false>(a, rp, st);
-    return per ? forward<float, true>(a, rp, st) : forward<float, false>(a, rp, st);
+    return GN_DISPATCH(forward_act, d.dtype, mode_of(s, es), a, res ? &r : nullptr, st);
 }
 
 int y5_launch_group_norm_bwd(const y5_group_norm_desc& d, hipStream_t st) {
@@ -848,9 +918,5 @@ int y5_launch_group_norm_bwd(const y5_group_norm_desc& d, hipStream_t st) {
     GnArgs a = make_args(d, s);
     a.part = static_cast<float2*>(d.workspace);
     a.cpart = reinterpret_cast<float*>(static_cast<char*>(d.workspace) + w.part);
-    const bool per = per_element(s, es);
-    const Resident* rp = res ? &r : nullptr;
-    if (d.dtype == Y5_F16) return per ? backward<f16, true>(a, rp, d.dweight, d.dbias, st) : backward<f16, false>(a, rp, d.dweight, d.dbias, st);
-    if (d.dtype == Y5_BF16) return per ? backward<bf16, true>(a, rp, d.dweight, d.dbias, st) : backward<bf16, false>(a, rp, d.dweight, d.dbias, st);
-    return per ? backward<float, true>(a, rp, d.dweight, d.dbias, st) : backward<float, false>(a, rp, d.dweight, d.dbias, st);
+    return GN_DISPATCH(backward_act, d.dtype, mode_of(s, es), a, res ? &r : nullptr, st);
 }

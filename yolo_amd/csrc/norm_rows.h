@@ -1,6 +1,6 @@
 // Pieces shared by the channels-last group norm (groupnorm.hip) and the 8-bit row quantisation (rows_i8.hip): element types,
 // 16-byte accesses at any element alignment, activations, and the group statistics that several chunks of an image left in
-// the workspace.  Included inside an anonymous namespace.
+// the workspace.  Included inside an anonymous namespace, after conv_common.h.
 #pragma once
 
 template <typename T>
@@ -57,6 +57,32 @@ __device__ __forceinline__ float ld_param(const void* p, int i, int dt, float de
     if (dt == Y5_F16) return (float)static_cast<const f16*>(p)[i];
     return (float)static_cast<const bf16*>(p)[i];
 }
+// N consecutive ones from element i on
+template <int N>
+__device__ __forceinline__ void ld_params(const void* p, int i, int dt, float def, float (&v)[N]) {
+    if (!p) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = def;
+    } else if (dt == Y5_F32) {
+#pragma unroll
+        for (int u = 0; u < N / 4; ++u) {
+            float w[4];
+            ld_vec(static_cast<const float*>(p) + i + 4 * u, w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * u + e] = w[e];
+        }
+    } else {
+        struct __attribute__((packed, aligned(2))) Half {
+            unsigned w[N / 2];
+        };
+        const Half h = *reinterpret_cast<const Half*>(static_cast<const unsigned short*>(p) + i);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const unsigned short b = (unsigned short)(h.w[e / 2] >> (16 * (e & 1)));
+            v[e] = dt == Y5_F16 ? (float)__builtin_bit_cast(f16, b) : __uint_as_float((unsigned)b << 16);
+        }
+    }
+}
 __device__ __forceinline__ void st_param(void* p, int i, int dt, float v) {
     if (dt == Y5_F32) static_cast<float*>(p)[i] = v;
     else if (dt == Y5_F16) static_cast<f16*>(p)[i] = (f16)v;
@@ -68,27 +94,26 @@ __device__ __forceinline__ void st_param(void* p, int i, int dt, float v) {
 __device__ __forceinline__ float norm_sigmoid(float z) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
 }
-template <int N>
-__device__ __forceinline__ void norm_act(float (&z)[N], int act, float slope) {
-    if (act == Y5_ACT_LEAKY) {
+// The activation is a template parameter (no activation is LeakyReLU of slope 1): a test at run time makes the compiler keep
+// several versions of everything around it.
+template <bool SILU, int N>
+__device__ __forceinline__ void norm_act(float (&z)[N], float slope) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) z[e] = z[e] > 0.f ? z[e] : z[e] * slope;
-    } else if (act == Y5_ACT_SILU) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) z[e] = z[e] * norm_sigmoid(z[e]);
+    for (int e = 0; e < N; ++e) {
+        if constexpr (SILU) z[e] = z[e] * norm_sigmoid(z[e]);
+        else z[e] = z[e] > 0.f ? z[e] : z[e] * slope;
     }
 }
 // d[e] *= act'(z[e])
-template <int N>
-__device__ __forceinline__ void norm_act_grad(float (&d)[N], const float (&z)[N], int act, float slope) {
-    if (act == Y5_ACT_LEAKY) {
+template <bool SILU, int N>
+__device__ __forceinline__ void norm_act_grad(float (&d)[N], const float (&z)[N], float slope) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) d[e] = z[e] > 0.f ? d[e] : d[e] * slope;
-    } else if (act == Y5_ACT_SILU) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
+    for (int e = 0; e < N; ++e) {
+        if constexpr (SILU) {
             const float p = norm_sigmoid(z[e]);
             d[e] *= p * __builtin_fmaf(z[e], 1.f - p, 1.f);
+        } else {
+            d[e] = z[e] > 0.f ? d[e] : d[e] * slope;
         }
     }
 }
@@ -106,6 +131,7 @@ struct NormShape {
     int batch;
     int act, param_dtype;
     float slope, eps;
+    FastDiv by_c, by_cpg, by_cols;
 };
 
 // pixels of chunk i of an image
@@ -162,7 +188,7 @@ __device__ __forceinline__ void norm_merge_chunks(const NormShape& s, const floa
 // ------------------------------------------------------------------------------------------ host
 
 constexpr int kNormMaxW = 4096;     // elements of a virtual row
-constexpr int kNormMaxChunks = 64;  // chunks of an image in the split form
+constexpr int kNormMaxChunks = 128;  // chunks of an image in the split form
 
 inline int norm_gcd(int a, int b) {
     while (b) {
@@ -197,15 +223,20 @@ inline int norm_make_shape(const y5_group_norm_desc& d, NormShape* out) {
     s.batch = d.batch;
     s.act = d.act;
     s.param_dtype = d.param_dtype;
-    s.slope = d.slope;
+    s.slope = d.act == Y5_ACT_LEAKY ? d.slope : 1.f;
     s.eps = d.eps;
-    // Chunks of the split form: 32 KiB of the tensor each, so that a chunk's reading hides its own reductions, at most
-    // kNormMaxChunks of an image (the second pass reads all of them in every workgroup)
+    // Chunks of the split form: as many workgroups as the chip holds at a time (1024 of 256 threads: 105 MB of 32 images in 27 us; twice
+    // as many leave a second, emptier round and more to merge: 32 us), at least 8 KiB each, at most kNormMaxChunks of an image (every
+    // workgroup of the second pass reads all of them)
     const long long bytes = (long long)d.pixels * d.c * norm_elem_size(d.dtype);
-    long long chunks = bytes / (32 << 10);
-    chunks = chunks < 1 ? 1 : chunks > kNormMaxChunks ? kNormMaxChunks : chunks;
+    long long chunks = 1024 / d.batch < kNormMaxChunks ? 1024 / d.batch : kNormMaxChunks;
+    chunks = chunks < bytes / 8192 ? chunks : bytes / 8192;
+    chunks = chunks < 1 ? 1 : chunks;
     s.chunk_rows = (int)((s.vrows + chunks - 1) / chunks);
     s.chunks = (s.vrows + s.chunk_rows - 1) / s.chunk_rows;
+    s.by_c = make_fastdiv((unsigned)s.c);
+    s.by_cpg = make_fastdiv((unsigned)s.cpg);
+    s.by_cols = make_fastdiv((unsigned)s.cols);
     *out = s;
     return Y5_OK;
 }
@@ -215,6 +246,13 @@ inline int norm_check_pitch(const y5_group_norm_desc& d, const NormShape& s, con
     Y5_REQUIRE(ld >= d.c && (s.k == 1 || ld == d.c), "group_norm: %s pitch %d for %d channels (a pitch above the channels needs channels in whole 16-byte vectors)", what, ld, d.c);
     Y5_REQUIRE(reinterpret_cast<uintptr_t>(p) % norm_elem_size(d.dtype) == 0, "group_norm: misaligned %s", what);
     return Y5_OK;
+}
+
+// What a workgroup of the split form's second pass reads: 32 KiB (merging the chunks' statistics is then little beside it; 64 KiB: 56
+// instead of 52 us for the gradient of 105 MB, 128 KiB: 60), less where that would leave compute units without one
+inline long long norm_run_bytes(const NormShape& s, int esize) {
+    const long long each = (long long)s.batch * s.pixels * s.c * esize / 2048;
+    return each < 4096 ? 4096 : each > 32768 ? 32768 : each;
 }
 
 inline size_t norm_align16(size_t n) { return (n + 15) / 16 * 16; }

@@ -12,17 +12,28 @@ __device__ __forceinline__ float row_scale(unsigned bits, float* a) {
     return *a / 127.f;
 }
 
-// The whole number nearest to v * 127 / a.  fp32 values are scaled in 64 bits: their 24 digits leave no room for an error of
-// the multiplication, which would put values next to a half on its other side.  16-bit values have 13 digits of room.
+// The whole number nearest to v * 127 / a, as the low byte of a word (the rest of the word is not zero).  Adding 1.5 * 2^23 (2^52)
+// leaves the number, to nearest with ties to even, in the low bits of the mantissa: one instruction for rounding and
+// converting.  The product is rounded before that, not in one step with it: its rounding takes the error of 127 / a back where the
+// quotient is exactly a half, which 16-bit values make of a few in ten thousand, and those then go to even.  fp32 values are
+// scaled in 64 bits: their 24 digits leave no room for the error of 127 / a, which would put values next to a half on its other side.
 struct Inv32 {
     float f;
     __device__ __forceinline__ void set(float a, bool ok) { f = ok && a > 0.f ? 127.f / a : 0.f; }
-    __device__ __forceinline__ int operator()(float v) const { return (int)__builtin_rintf(v * f); }
+    __device__ __forceinline__ unsigned operator()(float v) const {
+#pragma clang fp contract(off)
+        const float t = v * f;
+        return __float_as_uint(t + 12582912.f);
+    }
 };
 struct Inv64 {
     double f;
     __device__ __forceinline__ void set(float a, bool ok) { f = ok && a > 0.f ? 127.0 / (double)a : 0.0; }
-    __device__ __forceinline__ int operator()(float v) const { return (int)__builtin_rint((double)v * f); }
+    __device__ __forceinline__ unsigned operator()(float v) const {
+#pragma clang fp contract(off)
+        const double t = (double)v * f;
+        return (unsigned)__builtin_bit_cast(unsigned long long, t + 6755399441055744.0);
+    }
 };
 template <typename T, bool NORM>
 struct InvOf {
@@ -39,7 +50,34 @@ __device__ __forceinline__ unsigned max_bits(unsigned top, float v) {
     return u > top ? u : top;
 }
 
-__device__ __forceinline__ int pack_bytes(int a, int b, int c, int d) {  // each in [-128, 127]
-    const unsigned lo = __builtin_amdgcn_perm((unsigned)b, (unsigned)a, 0x0c0c0400u), hi = __builtin_amdgcn_perm((unsigned)d, (unsigned)c, 0x0c0c0400u);
-    return (int)__builtin_amdgcn_perm(hi, lo, 0x05040100u);
+// The low bytes of four words; zeros for a row that is not fine
+__device__ __forceinline__ int pack_bytes(unsigned a, unsigned b, unsigned c, unsigned d, bool fine) {
+    const unsigned lo = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), hi = __builtin_amdgcn_perm(d, c, 0x0c0c0400u);
+    return fine ? (int)__builtin_amdgcn_perm(hi, lo, 0x05040100u) : 0;
+}
+
+// The largest of `top` over aligned groups of `lanes` lanes (a power of two), FROM of them known to hold the same already.  Moves between
+// lanes of 16 and swaps of rows, which cost an instruction each; a shuffle through LDS costs its latency.
+template <int CTRL>
+__device__ __forceinline__ unsigned max_moved(unsigned top) {
+    const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, CTRL, 0xf, 0xf, true);
+    return o > top ? o : top;
+}
+template <int FROM = 1>
+__device__ __forceinline__ unsigned max_over(unsigned top, int lanes) {
+    if (FROM < 2 && lanes > 1) top = max_moved<0xb1>(top);    // lane ^ 1
+    if (FROM < 4 && lanes > 2) top = max_moved<0x4e>(top);    // lane ^ 2
+    if (FROM < 8 && lanes > 4) top = max_moved<0x141>(top);   // mirrored in 8
+    if (FROM < 16 && lanes > 8) top = max_moved<0x140>(top);  // mirrored in 16
+#if defined(__HIP_DEVICE_COMPILE__)
+    if (lanes > 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+        top = r[0] > r[1] ? r[0] : r[1];
+    }
+    if (lanes > 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+        top = r[0] > r[1] ? r[0] : r[1];
+    }
+#endif
+    return top;
 }

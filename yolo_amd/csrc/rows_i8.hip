@@ -10,8 +10,11 @@
 
 namespace {
 
+#include "conv_common.h"
 #include "norm_rows.h"
 #include "quant_rows.h"
+
+enum { kPlain, kNormLeaky, kNormSilu };  // what happens to a value before it is quantised
 
 struct RowsArgs {
     const void* x;
@@ -27,76 +30,110 @@ struct RowsArgs {
     const void *weight, *bias;
 };
 
-// V bytes of a row
+// V bytes of a row, from the low bytes of v
 template <int V>
-__device__ __forceinline__ void st_bytes(signed char* p, const int (&v)[V]) {
-    if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(pack_bytes(v[0], v[1], v[2], v[3]), pack_bytes(v[4], v[5], v[6], v[7]));
-    else *reinterpret_cast<int*>(p) = pack_bytes(v[0], v[1], v[2], v[3]);
+__device__ __forceinline__ void st_bytes(signed char* p, const unsigned (&v)[V], bool fine) {
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(pack_bytes(v[0], v[1], v[2], v[3], fine), pack_bytes(v[4], v[5], v[6], v[7], fine));
+    else *reinterpret_cast<int*>(p) = pack_bytes(v[0], v[1], v[2], v[3], fine);
 }
 
 // Lanes share a row: vector v of lane l covers elements ((v * lanes) + l) * V.  NV vectors a lane.
 // grid: runs of `run` rows (x batch with NORM, where a workgroup's rows are pixels of one image)
 // LDS with NORM: red[2 * blockDim.x], gmean, grstd[groups], A[q_ld], B[q_ld] (z = x * A + B)
-template <typename T, bool NORM, int NV>
+template <typename T, int NORM, int NV>
 __global__ __launch_bounds__(256) void rows_kernel(const RowsArgs a) {
     constexpr int V = NormElem<T>::V;
     extern __shared__ float lds[];
     const int t = threadIdx.x, TB = blockDim.x;
-    const int l = t & (a.lanes - 1);
+    const int l = t & (a.lanes - 1), sub = t / a.lanes, step = TB / a.lanes;
     long long row0 = (long long)blockIdx.x * a.run, rows = a.rows, base = 0;
-    float* coef = nullptr;
-    if constexpr (NORM) {
-        const NormShape& s = a.s;
-        const int b = s.batch - 1 - blockIdx.y;  // from the end: the statistics pass read that last
+    int b = 0;
+    if constexpr (NORM != kPlain) {
+        b = a.s.batch - 1 - blockIdx.y;  // from the end: the statistics pass read that last
         row0 = (long long)(gridDim.x - 1 - blockIdx.x) * a.run;
-        rows = s.pixels;
-        base = (long long)b * s.pixels;
+        rows = a.s.pixels;
+        base = (long long)b * a.s.pixels;
+    }
+    const long long row1 = row0 + a.run < rows ? row0 + a.run : rows;
+    int off[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) off[v] = (v * a.lanes + l) * V;
+    norm_u32x4 raw[NV];  // the values as they are in memory
+    auto load = [&](long long row) {
+        const T* xr = static_cast<const T*>(a.x) + (base + row) * a.x_ld;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int n = row < row1 ? a.k - off[v] : 0;
+            if (n >= V) raw[v] = reinterpret_cast<const NormVec<T>*>(xr + off[v])->v;
+            else {
+                NormArr<T> u;
+                ld_part(xr + off[v], n, u.v);
+                raw[v] = __builtin_bit_cast(norm_u32x4, u);
+            }
+        }
+    };
+    auto unpack = [&](int v) {  // the empty statement keeps the compiler from holding the values unpacked
+        asm volatile("" : "+v"(raw[v]));
+        return __builtin_bit_cast(NormArr<T>, raw[v]);
+    };
+    if constexpr (NORM != kPlain) load(row0 + sub);  // on its way while the statistics are merged
+    // up to two vectors a lane the coefficients live in registers (from LDS they would cost eight times the bytes of the values)
+    constexpr bool HELD = NORM != kPlain && NV <= 2;
+    float* coef = nullptr;
+    float A[HELD ? NV : 1][V], B[HELD ? NV : 1][V];
+    if constexpr (NORM != kPlain) {
+        const NormShape& s = a.s;
         float *red = lds, *gmean = red + 2 * TB, *grstd = gmean + s.groups;
         coef = grstd + s.groups;
+        float w0[2], b0[2];  // the first parameters too
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int c = t + i * TB;
+            w0[i] = c < s.c ? ld_param(a.weight, c, s.param_dtype, 1.f) : 0.f;
+            b0[i] = c < s.c ? ld_param(a.bias, c, s.param_dtype, 0.f) : 0.f;
+        }
         norm_merge_chunks(s, a.part, b, red, gmean, grstd);
         // mean and beta in one number: what that costs (the mean's magnitude over a deviation, times 2^-24) is far below the
         // 2^-8 of the rounding that follows
         for (int c = t; c < a.q_ld; c += TB) {
-            float A = 0.f, B = 0.f;
+            float ca = 0.f, cb = 0.f;
             if (c < s.c) {
-                const int g = c / s.cpg;
-                A = ld_param(a.weight, c, s.param_dtype, 1.f) * grstd[g];
-                B = __builtin_fmaf(-gmean[g], A, ld_param(a.bias, c, s.param_dtype, 0.f));
+                const int g = (int)fdiv((unsigned)c, s.by_cpg);
+                const bool first = c < 2 * TB;
+                ca = (first ? w0[c >= TB] : ld_param(a.weight, c, s.param_dtype, 1.f)) * grstd[g];
+                cb = __builtin_fmaf(-gmean[g], ca, first ? b0[c >= TB] : ld_param(a.bias, c, s.param_dtype, 0.f));
             }
-            coef[c] = A;
-            coef[a.q_ld + c] = B;
+            coef[c] = ca;
+            coef[a.q_ld + c] = cb;
         }
         __syncthreads();
-    }
-    int off[NV];
+        if constexpr (HELD) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) off[v] = (v * a.lanes + l) * V;
-    const long long row1 = row0 + a.run < rows ? row0 + a.run : rows;
-    const int step = TB / a.lanes;
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    A[v][e] = off[v] < a.q_ld ? coef[off[v] + e] : 0.f;
+                    B[v][e] = off[v] < a.q_ld ? coef[a.q_ld + off[v] + e] : 0.f;
+                }
+        }
+    }
     // every lane of a wave takes every turn: a row of lanes past the end reads and writes nothing
     for (long long first = row0; first < row1; first += step) {
-        const long long row = first + t / a.lanes;
-        const bool on = row < row1;
-        const T* xr = static_cast<const T*>(a.x) + (base + row) * a.x_ld;
-        T x[NV][V];
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int n = on ? a.k - off[v] : 0;
-            if (n >= V) ld_vec(xr + off[v], x[v]);
-            else ld_part(xr + off[v], n, x[v]);
-        }
+        const long long row = first + sub;
+        if constexpr (NORM == kPlain) load(row);
         unsigned top = 0;
-        float z[NORM ? NV : 1][V];
+        float z[NORM != kPlain ? NV : 1][V];
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             float f[V];
+            const NormArr<T> x = unpack(v);
 #pragma unroll
-            for (int e = 0; e < V; ++e) f[e] = (float)x[v][e];
-            if constexpr (NORM) {
-                if (off[v] < a.q_ld) {
+            for (int e = 0; e < V; ++e) f[e] = (float)x.v[e];
+            if constexpr (NORM != kPlain) {
+                if (HELD || off[v] < a.q_ld) {
 #pragma unroll
-                    for (int e = 0; e < V; ++e) f[e] = __builtin_fmaf(f[e], coef[off[v] + e], coef[a.q_ld + off[v] + e]);
-                    norm_act(f, a.s.act, a.s.slope);
+                    for (int e = 0; e < V; ++e) f[e] = HELD ? __builtin_fmaf(f[e], A[HELD ? v : 0][e], B[HELD ? v : 0][e]) : __builtin_fmaf(f[e], coef[off[v] + e], coef[a.q_ld + off[v] + e]);
+                    norm_act<NORM == kNormSilu>(f, a.s.slope);
                 }
 #pragma unroll
                 for (int e = 0; e < V; ++e) z[v][e] = f[e];
@@ -104,25 +141,25 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsArgs a) {
 #pragma unroll
             for (int e = 0; e < V; ++e) top = max_bits(top, f[e]);
         }
-        for (int d = a.lanes >> 1; d; d >>= 1) {
-            const unsigned u = (unsigned)__shfl_xor((int)top, d);
-            top = u > top ? u : top;
-        }
+        if constexpr (NORM != kPlain) load(row + step);  // the values are in z: the next row flies under the rest
+        top = max_over(top, a.lanes);
         float m;
         const float scale = row_scale(top, &m);
-        typename InvOf<T, NORM>::type inv;
+        typename InvOf<T, NORM != kPlain>::type inv;
         inv.set(m, top < 0x7f800000u);
-        if (!on) continue;
-        signed char* qr = a.q + (size_t)(base + row) * a.q_ld;
+        if (row < row1) {
+            signed char* qr = a.q + (size_t)(base + row) * a.q_ld;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            if (off[v] >= a.q_ld) continue;
-            int w[V];
+            for (int v = 0; v < NV; ++v) {
+                if (off[v] >= a.q_ld) continue;
+                unsigned w[V];
+                const NormArr<T> x = unpack(v);
 #pragma unroll
-            for (int e = 0; e < V; ++e) w[e] = top < 0x7f800000u ? inv(NORM ? z[NORM ? v : 0][e] : (float)x[v][e]) : 0;
-            st_bytes<V>(qr + off[v], w);
+                for (int e = 0; e < V; ++e) w[e] = inv(NORM != kPlain ? z[NORM != kPlain ? v : 0][e] : (float)x.v[e]);
+                st_bytes<V>(qr + off[v], w, top < 0x7f800000u);
+            }
+            if (l == 0) a.scale[base + row] = scale;
         }
-        if (l == 0) a.scale[base + row] = scale;
     }
 }
 
@@ -142,10 +179,7 @@ __global__ __launch_bounds__(256) void long_rows_kernel(const RowsArgs a) {
 #pragma unroll
         for (int e = 0; e < V; ++e) top = max_bits(top, (float)x[e]);
     }
-    for (int d = 32; d; d >>= 1) {
-        const unsigned u = (unsigned)__shfl_xor((int)top, d);
-        top = u > top ? u : top;
-    }
+    top = max_over(top, 64);
     if ((t & 63) == 0) tops[t >> 6] = top;
     __syncthreads();
     top = tops[0];
@@ -159,10 +193,10 @@ __global__ __launch_bounds__(256) void long_rows_kernel(const RowsArgs a) {
         T x[V];
         if (a.k - off >= V) ld_vec(xr + off, x);
         else ld_part(xr + off, a.k - off, x);
-        int w[V];
+        unsigned w[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) w[e] = top < 0x7f800000u ? inv((float)x[e]) : 0;
-        st_bytes<V>(a.q + (size_t)row * a.q_ld + off, w);
+        for (int e = 0; e < V; ++e) w[e] = inv((float)x[e]);
+        st_bytes<V>(a.q + (size_t)row * a.q_ld + off, w, top < 0x7f800000u);
     }
     if (t == 0) a.scale[row] = scale;
 }
@@ -180,20 +214,20 @@ int quantize(RowsArgs a, hipStream_t st) {
     while (a.lanes < 64 && a.lanes < vecs) a.lanes *= 2;
     const int nv = (vecs + a.lanes - 1) / a.lanes;
     const int step = 256 / a.lanes;  // rows of a workgroup in one turn
-    // four turns a workgroup, fewer where that would leave the chip empty
-    int turns = 4;
+    // four turns a workgroup, fewer where that would leave the chip empty; rows of many vectors have enough in flight in one
+    int turns = nv > 2 ? 1 : 4;
     while (turns > 1 && a.rows / ((long long)step * turns) < 1024) turns /= 2;
     a.run = step * turns;
     const dim3 grid((unsigned)((a.rows + a.run - 1) / a.run));
-    if (nv == 1) hipLaunchKernelGGL((rows_kernel<T, false, 1>), grid, dim3(256), 0, st, a);
-    else if (nv == 2) hipLaunchKernelGGL((rows_kernel<T, false, 2>), grid, dim3(256), 0, st, a);
-    else if (nv <= 4) hipLaunchKernelGGL((rows_kernel<T, false, 4>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((rows_kernel<T, false, 8>), grid, dim3(256), 0, st, a);
+    if (nv == 1) hipLaunchKernelGGL((rows_kernel<T, kPlain, 1>), grid, dim3(256), 0, st, a);
+    else if (nv == 2) hipLaunchKernelGGL((rows_kernel<T, kPlain, 2>), grid, dim3(256), 0, st, a);
+    else if (nv <= 4) hipLaunchKernelGGL((rows_kernel<T, kPlain, 4>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((rows_kernel<T, kPlain, 8>), grid, dim3(256), 0, st, a);
     Y5_LAUNCH_CHECK("rows_kernel");
     return Y5_OK;
 }
 
-template <typename T>
+template <typename T, int NORM>
 int norm_rows(RowsArgs a, hipStream_t st) {
     constexpr int V = NormElem<T>::V;
     const int vecs = a.q_ld / V;
@@ -201,8 +235,7 @@ int norm_rows(RowsArgs a, hipStream_t st) {
     while (a.lanes < 64 && a.lanes < vecs) a.lanes *= 2;
     const int nv = (vecs + a.lanes - 1) / a.lanes;
     const int step = 256 / a.lanes;
-    // rows of a workgroup: 32 KiB of them, so that merging the statistics is little beside it
-    long long run = (32 << 10) / ((long long)a.k * (int)sizeof(T));
+    long long run = norm_run_bytes(a.s, (int)sizeof(T)) / ((long long)a.k * (int)sizeof(T));
     run = run < step ? step : run / step * step;
     a.run = (int)run;
     const dim3 grid((unsigned)((a.s.pixels + run - 1) / run), (unsigned)a.s.batch);
@@ -213,13 +246,13 @@ int norm_rows(RowsArgs a, hipStream_t st) {
         Y5_LAUNCH_CHECK("rows_kernel");
         return Y5_OK;
     };
-    if (nv == 1) return launch(rows_kernel<T, true, 1>);
-    if (nv == 2) return launch(rows_kernel<T, true, 2>);
-    if (nv <= 4) return launch(rows_kernel<T, true, 4>);
+    if (nv == 1) return launch(rows_kernel<T, NORM, 1>);
+    if (nv == 2) return launch(rows_kernel<T, NORM, 2>);
+    if (nv <= 4) return launch(rows_kernel<T, NORM, 4>);
     if constexpr (V == 4) {
-        if (nv > 8) return launch(rows_kernel<T, true, 16>);
+        if (nv > 8) return launch(rows_kernel<T, NORM, 16>);
     }
-    return launch(rows_kernel<T, true, 8>);
+    return launch(rows_kernel<T, NORM, 8>);
 }
 
 int check_rows(const char* name, const void* q, const void* scale, int k, int q_ld) {
@@ -270,7 +303,8 @@ int y5_launch_group_norm_rows(const y5_group_norm_desc& d, void* q, int q_ld, fl
     a.part = static_cast<const float2*>(d.workspace);
     a.weight = d.weight;
     a.bias = d.bias;
-    if (d.dtype == Y5_F16) return norm_rows<f16>(a, st);
-    if (d.dtype == Y5_BF16) return norm_rows<bf16>(a, st);
-    return norm_rows<float>(a, st);
+    const bool silu = d.act == Y5_ACT_SILU;
+    if (d.dtype == Y5_F16) return silu ? norm_rows<f16, kNormSilu>(a, st) : norm_rows<f16, kNormLeaky>(a, st);
+    if (d.dtype == Y5_BF16) return silu ? norm_rows<bf16, kNormSilu>(a, st) : norm_rows<bf16, kNormLeaky>(a, st);
+    return silu ? norm_rows<float, kNormSilu>(a, st) : norm_rows<float, kNormLeaky>(a, st);
 }

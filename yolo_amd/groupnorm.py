@@ -206,7 +206,7 @@ def group_norm_rows(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, s
     any rounding are quantised, with a scale a pixel.  Inference only."""
     from yolo_amd import int8
     _check(x, num_groups, weight, bias, eps, act)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         raise RuntimeError('group_norm_rows has no gradient: call it under torch.no_grad()')
     lead = (x.shape[0], *x.shape[2:])
     if not x.is_cuda or x.numel() == 0:
@@ -215,8 +215,10 @@ def group_norm_rows(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, s
         rows = int8.quantize_rows(z.movedim(1, -1))
         rows.dtype = x.dtype
         return rows
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
     if not _current(x):
         with torch.cuda.device(x.device):
             return group_norm_rows(x, num_groups, weight, bias, eps, act, slope)

@@ -14,6 +14,7 @@ A row x becomes whole numbers q = nearest(127 x / max|x|) and the scale max|x| /
 Inference only.  CPU tensors go through torch's own operators (sums in fp64, exact too).
 """
 import ctypes as C
+import math
 from functools import lru_cache
 
 import torch
@@ -46,9 +47,7 @@ class Int8Rows:
     @classmethod
     def empty(cls, lead, k, dtype, device):
         _check_k(k)
-        n = 1
-        for v in lead:
-            n *= v
+        n = math.prod(lead)
         return cls(torch.empty((n, row_bytes(k)), dtype=torch.int8, device=device),
                    torch.empty(n, dtype=torch.float32, device=device), lead, k, dtype)
 
@@ -171,15 +170,15 @@ def _desc(q, scale, weight, bias, act, slope, y, m):
 
 
 def _product(rows, weight, bias, act, slope, dtype):
-    """(rows, n) of dtype from Int8Rows."""
+    """(*lead, n) of dtype from Int8Rows."""
     q = rows.q
     m = q.shape[0]
     if not q.is_cuda or m == 0:
-        return _plain_product(rows, weight, bias, act, slope, dtype)
+        return _plain_product(rows, weight, bias, act, slope, dtype).reshape(*rows.lead, weight.n)
     if not _current(q):
         with torch.cuda.device(q.device):
             return _product(rows, weight, bias, act, slope, dtype)
-    y = torch.empty((m, weight.n), dtype=dtype, device=q.device)
+    y = torch.empty((*rows.lead, weight.n), dtype=dtype, device=q.device)
     d = _desc(q.data_ptr(), rows.scale.data_ptr(), weight, bias, act, slope, y, m)
     rc = _lib.lib().y5_gemm_i8(C.byref(d), _lib.raw_stream(q.device.index))
     if rc:
@@ -241,7 +240,7 @@ def linear_i8(x, weight, bias=None, act=None, slope=0.1, dtype=None):
     if k != weight.k:
         raise ValueError('rows of %d values, weights for %d' % (k, weight.k))
     if rows:
-        return _product(x, weight, bias, act, slope, dtype).reshape(*x.lead, weight.n)
+        return _product(x, weight, bias, act, slope, dtype)
     if x.dtype not in _DTYPES:
         raise TypeError('linear_i8 expects fp16, bf16, fp32 or Int8Rows, got %s' % x.dtype)
     if x.requires_grad:
