@@ -424,7 +424,7 @@ int y5_nms_boxes_f32(const float* boxes, const float* scores, int n, double iou_
  * Tensors are (batch, pixels, c) with pixel pitch *_ld and images pixels * ld apart.  Any channel count c that the groups
  * divide; a pitch above c needs c in whole 16-byte vectors (multiples of 8, fp32: 4).  Pointers at element alignment.
  * Limit: c * (V / gcd(c, V)) <= 4096 with V = 8 (fp32: 4) values of a 16-byte vector.
- * y may be x; dx may be dy or x.  A group with an infinity or a NaN gives NaN throughout, other groups are untouched by it.
+ * At most 65535 images of at most 2^30 pixels.  y may be x; dx may be dy or x (other overlaps are not allowed).  A group with an infinity or a NaN gives NaN throughout, other groups are untouched by it.
  * Sums are taken in a fixed order: the same call gives the same bits.
  * ------------------------------------------------------------------------------------------ */
 typedef struct y5_group_norm_desc {
@@ -477,7 +477,7 @@ typedef struct y5_gemm_i8_desc {
     const void* w;        /* int8 [n][ld] */
     const float* w_scale; /* [n] */
     const float* bias;    /* [n] or NULL */
-    void* y;              /* [m] rows of n values of dtype at pitch y_ld, at element alignment */
+    void* y;              /* [m] rows of n values of dtype at pitch y_ld, at element alignment; overlaps no input */
     int64_t m, y_ld;
     int32_t n, k, ld;     /* ld = (k + 15) / 16 * 16 */
     int32_t dtype;        /* Y5_F16, Y5_BF16, Y5_F32 */

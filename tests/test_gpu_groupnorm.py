@@ -36,7 +36,7 @@ SHAPES = [
     ((1, 512, 20, 20), 32), ((2, 32, 64, 64), 1), ((2, 64, 17, 19), 32), ((2, 24, 9, 5), 8), ((3, 3, 181, 179), 1), ((2, 160, 13, 11), 32),
     ((2, 64, 80, 80), 32), ((1, 128, 80, 81), 32), ((1, 96, 101, 99), 4), ((1, 160, 90, 80), 32), ((2, 5, 199, 201), 5), ((2, 2, 300, 301), 1),
     ((1, 4096, 3, 3), 32), ((1, 4096, 2, 30), 4096), ((2, 511, 3, 5), 7), ((1, 1280, 25, 40), 32), ((1, 2, 2, 3, 4), 2), ((2, 16, 40, 33), 1),
-    ((1, 1024, 1, 1), 32), ((5, 8, 1, 37), 8), ((1, 4000, 40, 41), 1),
+    ((1, 1024, 1, 1), 32), ((5, 8, 1, 37), 8), ((1, 4000, 40, 41), 1), ((1, 4096, 40, 41), 4096), ((1, 4096, 33, 31), 512), ((2, 512, 90, 3), 512), ((300, 24, 1, 2), 3),
 ]
 
 

@@ -77,7 +77,7 @@ def product_ref(q, scale, w, wscale, bias, act, slope):
 # one token up to several tiles; long rows with few channels and the reverse
 PRODUCTS = [(1, 1, 1), (1, 16, 16), (2, 17, 3), (1, 4096, 512), (3, 1000, 255), (16, 64, 64), (17, 65, 33), (64, 128, 128), (65, 129, 257), (333, 1000, 255),
             (300, 80, 72), (1000, 32, 64), (515, 256, 256), (129, 2048, 130), (8, 20000, 24), (4, 640, 4100), (2049, 63, 40), (1030, 520, 392), (700, 1280, 700),
-            (20, 2048, 2064), (4100, 60, 130), (66000, 128, 72), (2000, 500, 2040), (4090, 512, 2048), (16300, 2000, 1000)]
+            (20, 2048, 2064), (4100, 60, 130), (66000, 128, 72), (2000, 500, 2040), (4090, 512, 2048), (16300, 2000, 1000), (1200000, 144, 1), (1060000, 16, 2)]
 
 
 @pytest.mark.parametrize('dtype', [F16, BF16, F32], ids=['fp16', 'bf16', 'fp32'])
@@ -246,6 +246,19 @@ def test_many_rows(dev):
     y = linear_i8(Int8Rows(q, torch.ones(m, device=dev), (m,), k, F16), w)
     assert torch.equal(y[idx], vals.half())
     assert int((y != 0).any(1).sum()) == int((vals != 0).any(1).sum())
+
+
+def test_one_row_and_scalars(dev):
+    w = quantize_weight(torch.randn(24, 40, generator=torch.Generator().manual_seed(1)).to(dev))
+    x = torch.randn(3, 40, generator=torch.Generator().manual_seed(2)).half().to(dev)
+    y = linear_i8(x, w)
+    assert torch.equal(linear_i8(x[1], w), y[1]) and linear_i8(x[1], w).shape == (24,)
+    assert torch.equal(linear_i8(quantize_rows(x[1]), w), y[1])
+    assert torch.equal(linear_i8(x[1].expand(5, 40), w), y[1].expand(5, 24))  # a pitch of zero
+    assert torch.equal(linear_i8(x.t().contiguous().t(), w), y)
+    one = Int8Weight(torch.full((3, 1), 5, dtype=torch.int8, device=dev), torch.ones(3, device=dev))
+    t = torch.tensor([[2.0], [-3.0], [0.0]], device=dev)
+    assert torch.allclose(linear_i8(t, one), (5 * t).expand(3, 3), rtol=1e-6)
 
 
 def test_empty(dev):

@@ -75,6 +75,11 @@ def test_refusals():
                  lambda: int8.Int8Conv1x1.from_conv(torch.nn.Conv2d(8, 8, 3)), lambda: int8.Int8Conv1x1.from_conv(torch.nn.Conv2d(8, 8, 1, groups=2))):
         with pytest.raises(ValueError):
             call()
+    q = torch.zeros(3, 16, dtype=torch.int8)
+    for args in ((q, torch.ones(4), (3,), 8), (q[:, :8], torch.ones(3), (3,), 8), (q, torch.ones(3), (2,), 8), (q, torch.ones(3), (3,), 17),
+                 (q, torch.ones(3).half(), (3,), 8), (q.float(), torch.ones(3), (3,), 8)):
+        with pytest.raises(ValueError):
+            int8.Int8Rows(*args, torch.float16)
     for call in (lambda: int8.linear_i8(t, torch.ones(4, 8)), lambda: int8.linear_i8(t.long(), w), lambda: int8.linear_i8(t, w, dtype=torch.float64),
                  lambda: int8.Int8Weight(torch.ones(4, 8), torch.ones(4)), lambda: int8.quantize_rows(t.double())):
         with pytest.raises(TypeError):

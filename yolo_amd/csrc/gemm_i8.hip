@@ -366,7 +366,7 @@ int y5_launch_gemm_i8(const y5_gemm_i8_desc& d, hipStream_t st) {
     if (y5_gemm_rows_fits(d.n, d.k, false, d.dtype) && ((d.k <= 64 && d.m >= 4096) || (d.k <= 128 && d.m >= 65536))) return y5_launch_gemm_rows(d, nullptr, 0, st);
     const GemmArgs g = make_gemm_args(d);
     const float few = few_cost(g, 16), few2 = few_cost(g, 32);
-    if ((few < few2 ? few : few2) < ph_cost(g, kPhTiles[best_ph(g)])) return y5_launch_gemm_few(d, nullptr, 0, few < few2 ? 16 : 32, st);
+    if (d.m <= 1 << 20 && (few < few2 ? few : few2) < ph_cost(g, kPhTiles[best_ph(g)])) return y5_launch_gemm_few(d, nullptr, 0, few < few2 ? 16 : 32, st);
     if (d.dtype == Y5_F16) return gemm_act<f16>(g, st);
     if (d.dtype == Y5_BF16) return gemm_act<bf16>(g, st);
     return gemm_act<float>(g, st);

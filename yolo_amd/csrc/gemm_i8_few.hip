@@ -21,6 +21,7 @@ struct FewArgs {
     const void* x;  // rows in their own type at pitch x_ld, k values each
     long long x_ld;
     int k;
+    int tiles_n;  // workgroups side by side
 };
 
 // Rows to 8 bits in LDS: q[row][ld], scale[row].  tops: LDS, one word a row, zero.
@@ -76,8 +77,9 @@ __global__ __launch_bounds__(kWaves * 64) void gemm_few_kernel(const FewArgs a) 
     const GemmArgs& g = a.g;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int lr = lane & 15, lq = lane >> 4;
-    const long long m0 = (long long)blockIdx.y * (16 * MI);
-    const int n0 = blockIdx.x * (16 * NI);
+    const int wm = blockIdx.x / a.tiles_n;
+    const long long m0 = (long long)wm * (16 * MI);
+    const int n0 = (blockIdx.x - wm * a.tiles_n) * (16 * NI);
     i32x4(*part)[MI * NI][64] = reinterpret_cast<i32x4(*)[MI * NI][64]>(smem);
     unsigned char* q = smem + (kWaves - 1) * MI * NI * 1024;
     const signed char *pa[MI], *pw[NI];
@@ -173,9 +175,11 @@ __global__ __launch_bounds__(kWaves * 64) void gemm_few_kernel(const FewArgs a) 
 }
 
 template <typename TI, typename T, int ACT, int MI, int NI>
-int launch(const FewArgs& a, hipStream_t st) {
-    const dim3 grid((unsigned)((a.g.n + 16 * NI - 1) / (16 * NI)), (unsigned)((a.g.m + 16 * MI - 1) / (16 * MI)));
-    Y5_REQUIRE(grid.y <= 65535, "gemm_i8: internal: %lld rows", a.g.m);
+int launch(FewArgs a, hipStream_t st) {
+    a.tiles_n = (a.g.n + 16 * NI - 1) / (16 * NI);
+    const long long total = (a.g.m + 16 * MI - 1) / (16 * MI) * a.tiles_n;
+    Y5_REQUIRE(total <= 0x7fffffffLL, "gemm_i8: %lld tiles", total);
+    const dim3 grid((unsigned)total);
     const size_t lds = (size_t)(kWaves - 1) * MI * NI * 1024 + (a.x ? (size_t)a.g.m * a.g.ld : 0);
     if (lds + 64 > 64 << 10) Y5_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_few_kernel<TI, T, ACT, MI, NI>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     hipLaunchKernelGGL((gemm_few_kernel<TI, T, ACT, MI, NI>), grid, dim3(kWaves * 64), lds, st, a);

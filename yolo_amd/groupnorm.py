@@ -12,7 +12,7 @@ included); another layout is copied to channels_last first.  The result is chann
 rounding at the end; sums are taken in a fixed order.  CPU tensors go through torch's own operators.
 
 Channels: any number the groups divide, up to 4096 (multiples of 8; multiples of 4 in fp32); at a lesser divisibility up to
-4096 / (8 / gcd(channels, 8)), e.g. 512 for odd counts in 16 bits.
+4096 / (8 / gcd(channels, 8)), e.g. 512 for odd counts in 16 bits.  Up to 65535 images of up to 2^30 pixels.
 """
 import ctypes as C
 from functools import lru_cache

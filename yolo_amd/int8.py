@@ -42,14 +42,26 @@ class Int8Rows:
     __slots__ = ('q', 'scale', 'lead', 'k', 'dtype')
 
     def __init__(self, q, scale, lead, k, dtype):
+        _check_k(k)
+        n = math.prod(lead)
+        if q.dtype is not torch.int8 or q.shape != (n, row_bytes(k)) or not q.is_contiguous():
+            raise ValueError('Int8Rows expects q as %d contiguous int8 rows of %d bytes, got %s %s' % (n, row_bytes(k), tuple(q.shape), q.dtype))
+        if scale.dtype is not torch.float32 or scale.shape != (n,) or not scale.is_contiguous() or scale.device != q.device:
+            raise ValueError('Int8Rows expects %d contiguous fp32 scales beside q, got %s %s' % (n, tuple(scale.shape), scale.dtype))
+        if dtype not in _DTYPES:
+            raise TypeError('Int8Rows stands for fp16, bf16 or fp32, not %s' % dtype)
         self.q, self.scale, self.lead, self.k, self.dtype = q, scale, tuple(lead), k, dtype
 
     @classmethod
     def empty(cls, lead, k, dtype, device):
+        """Rows to be filled."""
         _check_k(k)
         n = math.prod(lead)
-        return cls(torch.empty((n, row_bytes(k)), dtype=torch.int8, device=device),
-                   torch.empty(n, dtype=torch.float32, device=device), lead, k, dtype)
+        self = cls.__new__(cls)
+        self.q = torch.empty((n, row_bytes(k)), dtype=torch.int8, device=device)
+        self.scale = torch.empty(n, dtype=torch.float32, device=device)
+        self.lead, self.k, self.dtype = tuple(lead), k, dtype
+        return self
 
     @property
     def shape(self):
