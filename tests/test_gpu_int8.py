@@ -77,7 +77,7 @@ def product_ref(q, scale, w, wscale, bias, act, slope):
 # one token up to several tiles; long rows with few channels and the reverse
 PRODUCTS = [(1, 1, 1), (1, 16, 16), (2, 17, 3), (1, 4096, 512), (3, 1000, 255), (16, 64, 64), (17, 65, 33), (64, 128, 128), (65, 129, 257), (333, 1000, 255),
             (300, 80, 72), (1000, 32, 64), (515, 256, 256), (129, 2048, 130), (8, 20000, 24), (4, 640, 4100), (2049, 63, 40), (1030, 520, 392), (700, 1280, 700),
-            (20, 2048, 2064), (4100, 60, 130), (66000, 128, 72), (2000, 500, 2040), (4090, 512, 2048), (16300, 2000, 1000), (1200000, 144, 1), (1060000, 16, 2)]
+            (20, 2048, 2064), (4100, 60, 130), (66000, 128, 72), (66000, 240, 80), (66000, 500, 33), (2000, 500, 2040), (4090, 512, 2048), (16300, 2000, 1000), (1200000, 144, 1), (1060000, 16, 2)]
 
 
 @pytest.mark.parametrize('dtype', [F16, BF16, F32], ids=['fp16', 'bf16', 'fp32'])
@@ -101,7 +101,7 @@ def test_product(dev, m, k, n, dtype):
 
 @pytest.mark.parametrize('dtype', [F16, BF16, F32], ids=['fp16', 'bf16', 'fp32'])
 @pytest.mark.parametrize('m,k,n', [(1, 4096, 96), (2, 30, 7), (5, 257, 300), (13, 1024, 64), (16, 640, 255), (31, 96, 17), (77, 200, 64), (900, 64, 64), (1111, 72, 24), (513, 512, 130), (640, 250, 256),
-                                   (2100, 48, 130), (17000, 128, 80), (16500, 240, 33), (16400, 512, 64), (16400, 256, 528), (16400, 272, 20), (4, 16384, 24), (3, 21848, 40)])
+                                   (4100, 48, 130), (17000, 128, 80), (16500, 240, 33), (16400, 512, 64), (16400, 256, 200), (16400, 272, 20), (4, 16384, 24), (3, 21848, 40)])
 def test_linear_from_floating_point(dev, m, k, n, dtype):
     """linear_i8 of a tensor is the product of its quantised rows: the same bits as in two calls, and those within tolerance."""
     g = torch.Generator().manual_seed(m * 7 + k + n)

@@ -360,10 +360,10 @@ int check(const y5_gemm_i8_desc& d) {
 int y5_launch_gemm_i8(const y5_gemm_i8_desc& d, hipStream_t st) {
     Y5_REQUIRE(d.a && d.a_scale, "gemm_i8: null tensor pointer");
     if (int rc = check(d)) return rc;
-    // Many rows of at most 128 values: the weights fit a corner of LDS and the tiles' fixed costs outweigh their reuse (819200 x 64
-    // x 64: 29 us against 38 - 84 of the tiles, 204800 x 128 x 256: 31 against 33, 51200 x 64 x 64: 4.5 against 6.3; but 51200 x 128 x
-    // 128: 7.9 against 7.8, 204800 x 256 x 128: 28 against 26)
-    if (y5_gemm_rows_fits(d.n, d.k, false, d.dtype) && ((d.k <= 64 && d.m >= 4096) || (d.k <= 128 && d.m >= 65536))) return y5_launch_gemm_rows(d, nullptr, 0, st);
+    // Many rows of few values: the weights fit LDS and the tiles' fixed costs outweigh their reuse (819200 x 64 x 64: 29 us against 53 of
+    // the best tile, 204800 x 256 x 64: 17 against 24, 204800 x 256 x 256: 37 against 40, 204800 x 512 x 128: 35 against 36, 51200 x 64 x
+    // 64: 4.6 against 6.4; but 51200 x 128 x 128: 7.4 against 7.6, 51200 x 512 x 128: 14 against 11, 12800 x 256 x 256: 8.8 against 5.8)
+    if (y5_gemm_rows_fits(d.n, d.k, false, d.dtype) && (d.m >= 65536 || (d.k <= 64 && d.m >= 4096))) return y5_launch_gemm_rows(d, nullptr, 0, st);
     const GemmArgs g = make_gemm_args(d);
     const float few = few_cost(g, 16), few2 = few_cost(g, 32);
     if (d.m <= 1 << 20 && (few < few2 ? few : few2) < ph_cost(g, kPhTiles[best_ph(g)])) return y5_launch_gemm_few(d, nullptr, 0, few < few2 ? 16 : 32, st);
@@ -378,11 +378,12 @@ namespace {
 enum { kTwoSteps, kFew, kRows };
 int fused(const y5_gemm_i8_desc& d, int x_dtype) {
     if (x_dtype != d.dtype) return kTwoSteps;
-    // 1 x 4096 x 4096: 6.3 us in one, 10.9 in two; 4 x 4096 x 4096: 9.7 and 11.5; every workgroup quantises all rows, so not more
+    // 1 x 4096 x 4096: 6.3 us in one, 10.9 in two; 4 x 4096 x 4096: 8.7 and 11.5; every workgroup quantises all rows, so not more
     if (d.m <= Y5_FEW_ROWS && d.m * d.ld <= 64 * 1024) return kFew;
-    // 2048 x 64 x 64: 5.3 us in one, 6.3 in two; 819200 x 64 x 64: 42 and 58; 12800 x 128 x 128: 8.6 and 7.8; 51200 x 128 x 128: 10.7
-    // and 16.4; 204800 x 512 x 64: 52 and 85
-    return d.m >= (d.k <= 64 ? 2048 : 16384) && y5_gemm_rows_fits(d.n, d.k, true, d.dtype) ? kRows : kTwoSteps;
+    // The one launch has the weights to lay out in every workgroup's LDS before its rows (4096 x 128 x 128: 5.3 us in one, 6.5 in two; 819200
+    // x 64 x 64: 39 and 55; 204800 x 256 x 256: 46 and 65; 12800 x 512 x 64: 9.1 and 13.1; but 12800 x 256 x 256: 10.7 and 10.8, 16384 x
+    // 512 x 256: 18.1 and 16.3, 2048 x 64 x 64 in fp32: 5.9 and 5.3)
+    return d.m >= 4096 && d.m >= (int64_t)d.n * d.k / 4 && y5_gemm_rows_fits(d.n, d.k, true, d.dtype) ? kRows : kTwoSteps;
 }
 }  // namespace
 

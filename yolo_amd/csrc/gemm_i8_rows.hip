@@ -26,14 +26,20 @@ struct RowsGemm {
 };
 
 template <typename TI>
-struct Frag {  // 16 values of a row as they are read
+struct Frag {  // 16 values of a row as they are in memory
     static constexpr int NV = (int)sizeof(TI);
-    TI v[NV][NormElem<TI>::V];
+    norm_u32x4 v[NV];
+    // the empty statement keeps the compiler from holding the values unpacked
+    __device__ __forceinline__ NormArr<TI> unpack(int u) {
+        asm volatile("" : "+v"(v[u]));
+        return __builtin_bit_cast(NormArr<TI>, v[u]);
+    }
 };
 
 template <typename TI, typename T, int ACT, int MI, int KF>
-__global__ __launch_bounds__(512, 2) void gemm_rows_kernel(const RowsGemm a) {
+__global__ __launch_bounds__(512, sizeof(TI) == 4 && KF == 4 ? 2 : 4) void gemm_rows_kernel(const RowsGemm a) {
     constexpr bool QUANT = sizeof(TI) != 1;
+    constexpr bool AHEAD = KF <= 4;  // the next block's values fly under this one's products; of 512 values a row there is no room for two
     constexpr int SV = 16 / (int)sizeof(T);
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     const GemmArgs& g = a.g;
@@ -73,11 +79,8 @@ __global__ __launch_bounds__(512, 2) void gemm_rows_kernel(const RowsGemm a) {
                     const bool in = row < g.m && k < a.k;
 #pragma unroll
                     for (int u = 0; u < Frag<TX>::NV; ++u) {
-                        if (in) ld_vec(p + u * NormElem<TX>::V, raw[i][f].v[u]);
-                        else {
-#pragma unroll
-                            for (int e = 0; e < NormElem<TX>::V; ++e) raw[i][f].v[u][e] = (TX)0.f;
-                        }
+                        raw[i][f].v[u] = norm_u32x4{0, 0, 0, 0};
+                        if (in) raw[i][f].v[u] = reinterpret_cast<const NormVec<TX>*>(p + u * NormElem<TX>::V)->v;
                     }
                 } else {
                     qn[i][f] = i32x4{0, 0, 0, 0};
@@ -88,8 +91,9 @@ __global__ __launch_bounds__(512, 2) void gemm_rows_kernel(const RowsGemm a) {
     };
     const long long stride = (long long)gridDim.x * 8;
     long long blk = (long long)blockIdx.x * 8 + wave;
-    if (blk < a.blocks) load(blk);
+    if (AHEAD && blk < a.blocks) load(blk);
     for (; blk < a.blocks; blk += stride) {
+        if constexpr (!AHEAD) load(blk);
         i32x4 q[MI][KF];
         float s[MI];
 #pragma unroll
@@ -99,9 +103,11 @@ __global__ __launch_bounds__(512, 2) void gemm_rows_kernel(const RowsGemm a) {
 #pragma unroll
                 for (int f = 0; f < KF; ++f)
 #pragma unroll
-                    for (int u = 0; u < Frag<TX>::NV; ++u)
+                    for (int u = 0; u < Frag<TX>::NV; ++u) {
+                        const NormArr<TX> x = raw[i][f].unpack(u);
 #pragma unroll
-                        for (int e = 0; e < NormElem<TX>::V; ++e) top = max_bits(top, (float)raw[i][f].v[u][e]);
+                        for (int e = 0; e < NormElem<TX>::V; ++e) top = max_bits(top, (float)x.v[e]);
+                    }
                 top = max_over<16>(top, 64);  // of the four lanes that share a row
                 const bool fine = top < 0x7f800000u;
                 float m;
@@ -112,9 +118,11 @@ __global__ __launch_bounds__(512, 2) void gemm_rows_kernel(const RowsGemm a) {
                 for (int f = 0; f < KF; ++f) {
                     unsigned w[16];
 #pragma unroll
-                    for (int u = 0; u < Frag<TX>::NV; ++u)
+                    for (int u = 0; u < Frag<TX>::NV; ++u) {
+                        const NormArr<TX> x = raw[i][f].unpack(u);
 #pragma unroll
-                        for (int e = 0; e < NormElem<TX>::V; ++e) w[u * NormElem<TX>::V + e] = inv((float)raw[i][f].v[u][e]);
+                        for (int e = 0; e < NormElem<TX>::V; ++e) w[u * NormElem<TX>::V + e] = inv((float)x.v[e]);
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) q[i][f][e] = pack_bytes(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3], fine);
                 }
@@ -124,7 +132,7 @@ __global__ __launch_bounds__(512, 2) void gemm_rows_kernel(const RowsGemm a) {
                 for (int f = 0; f < KF; ++f) q[i][f] = qn[i][f];
             }
         }
-        if (blk + stride < a.blocks) load(blk + stride);
+        if (AHEAD && blk + stride < a.blocks) load(blk + stride);
         for (int c = 0; c < a.chunks; ++c) {
             i32x4 acc[MI][4];
 #pragma unroll
@@ -196,8 +204,8 @@ int by_width(const RowsGemm& a, hipStream_t st) {
     const int kf = (a.k + 63) / 64;
     constexpr bool wide = sizeof(TI) == 4;  // fp32 values take twice the registers
     if (kf == 1) return launch<TI, T, ACT, 2, 1>(a, st);
-    if (kf == 2) return launch<TI, T, ACT, 2, 2>(a, st);
-    if (kf <= 4) return launch<TI, T, ACT, wide ? 1 : 2, 4>(a, st);
+    if (kf == 2) return launch<TI, T, ACT, 1, 2>(a, st);
+    if (kf <= 4) return launch<TI, T, ACT, 1, 4>(a, st);
     if constexpr (!wide) return launch<TI, T, ACT, 1, 8>(a, st);
     return y5_fail(Y5_EINVAL, "gemm_i8: internal: %d values a row", a.k);
 }
