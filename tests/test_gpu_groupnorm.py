@@ -220,6 +220,41 @@ def test_writes_only_its_own_channels(dev):
         assert bool((wide[..., :8] == 7).all()) and bool((wide[..., 24:] == 7).all())
 
 
+def test_differentiable_once(dev):
+    x, w, b, dy = (v.to(dev) for v in make((1, 8, 3, 2), F32, 41))
+    with torch.enable_grad():
+        leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+        plain = torch.autograd.grad(group_norm(leaves[0], 2, leaves[1], leaves[2], act='silu'), leaves, dy)
+        again = torch.autograd.grad(group_norm(leaves[0], 2, leaves[1], leaves[2], act='silu'), leaves, dy, create_graph=True)
+        assert all(torch.equal(p, q) for p, q in zip(plain, again))
+        with pytest.raises(RuntimeError, match='differentiable once'):
+            again[0].sum().backward()
+        y = group_norm(leaves[0], 2, leaves[1], leaves[2])
+        with torch.no_grad():
+            leaves[0].mul_(2)
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            y.sum().backward()
+
+
+def test_errors_of_the_library_and_leaf_gradients(dev):
+    with pytest.raises(_lib.Y5Error, match='channels'):
+        group_norm(torch.zeros(1, 513, 2, 2, dtype=F16, device=dev), 1)
+    with pytest.raises(_lib.Y5Error, match='batch'):
+        group_norm(torch.zeros(65536, 8, dtype=F16, device=dev), 1)
+    # gradients accumulate on leaves of several layouts; bias alone, weight alone
+    x, w, b, dy = (v.to(dev) for v in make((2, 24, 5, 4), F16, 43))
+    want = torch.autograd.grad
+    for need in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1), (0, 1, 1)):
+        with torch.enable_grad():
+            leaves = [v.detach().clone().requires_grad_(bool(n)) for v, n in zip((x, w, b), need)]
+            full = [v.detach().clone().requires_grad_() for v in (x, w, b)]
+            grads = want(group_norm(full[0], 4, full[1], full[2], act='leaky'), full, dy)
+            for _ in range(2):
+                group_norm(leaves[0], 4, leaves[1], leaves[2], act='leaky').backward(dy.contiguous())
+        for leaf, n, g in zip(leaves, need, grads):
+            assert (leaf.grad is not None) == bool(n) and (not n or torch.equal(leaf.grad, g + g))
+
+
 def test_empty_and_module(dev):
     for shape in ((0, 8, 3, 3), (2, 8, 0, 3)):
         with torch.enable_grad():

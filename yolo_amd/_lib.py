@@ -5,7 +5,6 @@ fallback: if it is missing, every GPU entry point of this package raises.
 """
 import ctypes as C
 import os
-import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'liby5hip.so')
@@ -75,19 +74,6 @@ class GemmI8Desc(C.Structure):
     _fields_ = [('a', C.c_void_p), ('a_scale', C.c_void_p), ('w', C.c_void_p), ('w_scale', C.c_void_p), ('bias', C.c_void_p),
                 ('y', C.c_void_p), ('m', C.c_int64), ('y_ld', C.c_int64), ('n', C.c_int32), ('k', C.c_int32), ('ld', C.c_int32),
                 ('dtype', C.c_int32), ('act', C.c_int32), ('slope', C.c_float)]
-
-
-# The descriptors of the per-call entry points, filled in one step: setting two dozen ctypes fields one by one costs more host time
-# than a small launch.  Arguments in field order, 0 for a null pointer.
-_GN_PACK, _GEMM_PACK = struct.Struct('12Q11i2f4x'), struct.Struct('6Q2q5if')
-
-
-def group_norm_desc(*fields):
-    return GroupNormDesc.from_buffer_copy(_GN_PACK.pack(*fields))
-
-
-def gemm_i8_desc(*fields):
-    return GemmI8Desc.from_buffer_copy(_GEMM_PACK.pack(*fields))
 
 
 # name -> (restype, argtypes); every symbol include/y5hip.h declares
@@ -211,7 +197,19 @@ def current_stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def raw_stream(index):
-    """The current stream of device `index`, as the entry points take it."""
-    import torch
-    return torch._C._cuda_getCurrentRawStream(index)
+_calls = None
+
+
+def calls():
+    """The extension module _calls.so: the per-call host side of groupnorm and int8 (same build, same rule as lib())."""
+    global _calls
+    if _calls is None:
+        lib()
+        try:
+            from yolo_amd import _calls as module
+        except ImportError as e:
+            raise Y5Error('yolo_amd/_calls.so could not be loaded (%s) - build it with `make -C yolo_amd/csrc`; the GPU path has no '
+                          'fallback' % e) from e
+        module.raise_as(Y5Error)
+        _calls = module
+    return _calls

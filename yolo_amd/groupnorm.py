@@ -14,12 +14,8 @@ rounding at the end; sums are taken in a fixed order.  CPU tensors go through to
 Channels: any number the groups divide, up to 4096 (multiples of 8; multiples of 4 in fp32); at a lesser divisibility up to
 4096 / (8 / gcd(channels, 8)), e.g. 512 for odd counts in 16 bits.  Up to 65535 images of up to 2^30 pixels.
 """
-import ctypes as C
-from functools import lru_cache
-
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from yolo_amd import _lib
 
@@ -69,17 +65,6 @@ def channels_last(x):
     return x, pitch
 
 
-def empty_like_channels_last(x):
-    if x.dim() == 4 and x.is_contiguous(memory_format=torch.channels_last):
-        return torch.empty_like(x)
-    return torch.empty((x.shape[0], *x.shape[2:], x.shape[1]), dtype=x.dtype, device=x.device).movedim(-1, 1)
-
-
-def _current(x):
-    """Whether x's device is the current one."""
-    return x.device.index == torch.cuda.current_device()
-
-
 def _check(x, num_groups, weight, bias, eps, act):
     if x.dim() < 2:
         raise ValueError('group_norm expects (batch, channels, ...), got shape %s' % (tuple(x.shape),))
@@ -112,79 +97,6 @@ def _plain(x, num_groups, weight, bias, eps, act, slope):
     return y.movedim(1, -1).contiguous().movedim(-1, 1)
 
 
-@lru_cache(maxsize=4096)
-def _workspace_bytes(what, batch, pixels, c, groups, dtype, param_dtype):
-    d = _lib.group_norm_desc(*(0,) * 12, batch, pixels, c, groups, c, c, c, c, dtype, param_dtype, 0, 0.0, 0.0)
-    n = C.c_size_t()
-    _lib.check(_lib.lib().y5_group_norm_workspace(C.byref(d), what, C.byref(n)))
-    return n.value
-
-
-def _run(what, x, pitch, groups, weight, bias, eps, act, slope, y=0, dy=0, dy_ld=0, dx=0, dweight=0, dbias=0, stats=0, rows=None):
-    """One of the three calls on x's (current) device and its current stream.  stats: address of (2, batch, groups) fp32."""
-    batch, c = x.shape[0], x.shape[1]
-    pixels = x.numel() // (batch * c)
-    p = weight if weight is not None else bias
-    dtype, param_dtype = _DTYPES[x.dtype], _lib.F32 if p is None else _DTYPES[p.dtype]
-    n = _workspace_bytes(what, batch, pixels, c, groups, dtype, param_dtype)
-    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    d = _lib.group_norm_desc(x.data_ptr(), y, dy, dx, 0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
-                             dweight, dbias, stats, stats and stats + 4 * batch * groups, 0 if ws is None else ws.data_ptr(), n, batch, pixels, c,
-                             groups, pitch, c, dy_ld, c, dtype, param_dtype, _ACTS[act], slope, eps)
-    lib, stream = _lib.lib(), _lib.raw_stream(x.device.index)
-    if what == _lib.GN_FORWARD:
-        rc = lib.y5_group_norm(C.byref(d), stream)
-    elif what == _lib.GN_BACKWARD:
-        rc = lib.y5_group_norm_backward(C.byref(d), stream)
-    else:
-        rc = lib.y5_group_norm_rows_i8(C.byref(d), rows.q.data_ptr(), rows.q.shape[1], rows.scale.data_ptr(), stream)
-    if rc:
-        _lib.check(rc)
-
-
-def _forward(x, num_groups, weight, bias, eps, act, slope, want_stats):
-    """(y, x as it was read, (2, batch, groups) mean and 1 / deviation or None)."""
-    if not _current(x):
-        with torch.cuda.device(x.device):
-            return _forward(x, num_groups, weight, bias, eps, act, slope, want_stats)
-    x, pitch = channels_last(x)
-    y = empty_like_channels_last(x)
-    stats = torch.empty((2, x.shape[0], num_groups), dtype=torch.float32, device=x.device) if want_stats else None
-    _run(_lib.GN_FORWARD, x, pitch, num_groups, weight, bias, eps, act, slope, y=y.data_ptr(), stats=0 if stats is None else stats.data_ptr())
-    return y, x, stats
-
-
-class _GroupNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, *args):
-        y, xl, stats = _forward(x, args[0], weight, bias, *args[1:], True)
-        ctx.save_for_backward(xl, weight, bias, stats)
-        ctx.args = args
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
-        if not _current(x):
-            with torch.cuda.device(x.device):
-                return _backward(ctx, x, weight, bias, stats, dy)
-        return _backward(ctx, x, weight, bias, stats, dy)
-
-
-def _backward(ctx, x, weight, bias, stats, dy):
-    need = ctx.needs_input_grad
-    dy, dy_ld = channels_last(dy)
-    dx = empty_like_channels_last(x) if need[0] else None
-    dw = torch.empty_like(weight) if need[1] else None
-    db = torch.empty_like(bias) if need[2] else None
-    num_groups, eps, act, slope = ctx.args
-    _run(_lib.GN_BACKWARD, x, channels_last(x)[1], num_groups, weight, bias, eps, act, slope, dy=dy.data_ptr(), dy_ld=dy_ld,
-         dx=0 if dx is None else dx.data_ptr(), dweight=0 if dw is None else dw.data_ptr(), dbias=0 if db is None else db.data_ptr(),
-         stats=stats.data_ptr())
-    return dx, dw, db, None, None, None, None
-
-
 def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, slope=0.1):
     """act(group_norm(x)) in x's type, channels_last.  weight, bias: (channels,) of one type (x's, or fp32 beside a 16-bit x),
     or None.  act: None, 'leaky' (with slope) or 'silu'.  Differentiable once in x, weight and bias; their gradients
@@ -196,9 +108,8 @@ def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, slope=
         weight = weight.contiguous()
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
-        return _GroupNorm.apply(x, weight, bias, num_groups, eps, act, slope)
-    return _forward(x, num_groups, weight, bias, eps, act, slope, False)[0]
+    x, pitch = channels_last(x)
+    return _lib.calls().group_norm(x, pitch, num_groups, weight, bias, eps, _ACTS[act], slope)
 
 
 def group_norm_rows(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, slope=0.1):
@@ -219,13 +130,9 @@ def group_norm_rows(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, s
         weight = weight.contiguous()
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    if not _current(x):
-        with torch.cuda.device(x.device):
-            return group_norm_rows(x, num_groups, weight, bias, eps, act, slope)
-    x, pitch = channels_last(x)
-    rows = int8.Int8Rows.empty(lead, x.shape[1], x.dtype, x.device)
-    _run(_lib.GN_ROWS, x, pitch, num_groups, weight, bias, eps, act, slope, rows=rows)
-    return rows
+    xl, pitch = channels_last(x)
+    q, scale = _lib.calls().group_norm_rows(xl, pitch, num_groups, weight, bias, eps, _ACTS[act], slope)
+    return int8.Int8Rows.of(q, scale, lead, x.shape[1], x.dtype)
 
 
 class GroupNormAct(nn.GroupNorm):

@@ -13,15 +13,13 @@ A row x becomes whole numbers q = nearest(127 x / max|x|) and the scale max|x| /
 0; a row with an infinity or a NaN gives NaN outputs.  y = act(sum(q w) * (scale_row * scale_channel) + bias) in fp32, rounded once.
 Inference only.  CPU tensors go through torch's own operators (sums in fp64, exact too).
 """
-import ctypes as C
 import math
-from functools import lru_cache
 
 import torch
 import torch.nn as nn
 
 from yolo_amd import _lib
-from yolo_amd.groupnorm import _ACTS, _DTYPES, _current, act_code, apply_act, pixel_pitch
+from yolo_amd.groupnorm import _ACTS, _DTYPES, act_code, apply_act, pixel_pitch
 
 ZERO_ROW = 2.0 ** -120
 
@@ -53,14 +51,10 @@ class Int8Rows:
         self.q, self.scale, self.lead, self.k, self.dtype = q, scale, tuple(lead), k, dtype
 
     @classmethod
-    def empty(cls, lead, k, dtype, device):
-        """Rows to be filled."""
-        _check_k(k)
-        n = math.prod(lead)
+    def of(cls, q, scale, lead, k, dtype):
+        """What the kernels wrote, unchecked."""
         self = cls.__new__(cls)
-        self.q = torch.empty((n, row_bytes(k)), dtype=torch.int8, device=device)
-        self.scale = torch.empty(n, dtype=torch.float32, device=device)
-        self.lead, self.k, self.dtype = tuple(lead), k, dtype
+        self.q, self.scale, self.lead, self.k, self.dtype = q, scale, lead, k, dtype
         return self
 
     @property
@@ -123,17 +117,6 @@ def _quantize_plain(x, lead, k, dtype):
     return Int8Rows(torch.nn.functional.pad(q.to(torch.int8), (0, row_bytes(k) - k)), scale[:, 0].float(), lead, k, dtype)
 
 
-def _quantize(x, pitch, lead, k):
-    """x: any view whose rows of k values lie `pitch` elements apart."""
-    if not _current(x):
-        with torch.cuda.device(x.device):
-            return _quantize(x, pitch, lead, k)
-    rows = Int8Rows.empty(lead, k, x.dtype, x.device)
-    _lib.check(_lib.lib().y5_quantize_rows_i8(x.data_ptr(), pitch, _DTYPES[x.dtype], rows.q.shape[0], k, rows.q.data_ptr(),
-                                              rows.q.shape[1], rows.scale.data_ptr(), _lib.raw_stream(x.device.index)))
-    return rows
-
-
 def _rows_of(x):
     """x (..., k) as rows at one pitch: itself where its memory is that, else a copy."""
     k = x.shape[-1]
@@ -151,12 +134,12 @@ def quantize_rows(x):
     if x.dim() < 1:
         raise ValueError('quantize_rows expects (..., k)')
     _refuse_grad('quantize_rows', x)
-    lead, k = x.shape[:-1], x.shape[-1]
+    lead, k = tuple(x.shape[:-1]), x.shape[-1]
     _check_k(k)
     if not x.is_cuda or x.numel() == 0:
         return _quantize_plain(x, lead, k, x.dtype)
-    x, pitch = _rows_of(x)
-    return _quantize(x, pitch, lead, k)
+    r, pitch = _rows_of(x)
+    return Int8Rows.of(*_lib.calls().quantize_rows(r, pitch, r.shape[0], k), lead, k, x.dtype)
 
 
 def quantize_weight(w):
@@ -174,52 +157,6 @@ def _plain_product(rows, weight, bias, act, slope, dtype):
     y = y.float() * (rows.scale[:, None] * weight.scale)
     y = y if bias is None else y + bias
     return apply_act(y, act, slope).to(dtype)
-
-
-def _desc(q, scale, weight, bias, act, slope, y, m):
-    return _lib.gemm_i8_desc(q, scale, weight.q.data_ptr(), weight.scale.data_ptr(), 0 if bias is None else bias.data_ptr(), y.data_ptr(), m,
-                             weight.n, weight.n, weight.k, weight.q.shape[1], _DTYPES[y.dtype], _ACTS[act], slope)
-
-
-def _product(rows, weight, bias, act, slope, dtype):
-    """(*lead, n) of dtype from Int8Rows."""
-    q = rows.q
-    m = q.shape[0]
-    if not q.is_cuda or m == 0:
-        return _plain_product(rows, weight, bias, act, slope, dtype).reshape(*rows.lead, weight.n)
-    if not _current(q):
-        with torch.cuda.device(q.device):
-            return _product(rows, weight, bias, act, slope, dtype)
-    y = torch.empty((*rows.lead, weight.n), dtype=dtype, device=q.device)
-    d = _desc(q.data_ptr(), rows.scale.data_ptr(), weight, bias, act, slope, y, m)
-    rc = _lib.lib().y5_gemm_i8(C.byref(d), _lib.raw_stream(q.device.index))
-    if rc:
-        _lib.check(rc)
-    return y
-
-
-@lru_cache(maxsize=4096)
-def _workspace_bytes(m, n, k, dtype, x_dtype):
-    d = _lib.gemm_i8_desc(0, 0, 0, 0, 0, 0, m, n, n, k, row_bytes(k), dtype, 0, 0.0)
-    size = C.c_size_t()
-    _lib.check(_lib.lib().y5_linear_i8_workspace(C.byref(d), x_dtype, C.byref(size)))
-    return size.value
-
-
-def _linear(x, pitch, m, weight, bias, act, slope, dtype):
-    """(m, n) of dtype from m rows `pitch` elements apart, quantised on the way."""
-    if not _current(x):
-        with torch.cuda.device(x.device):
-            return _linear(x, pitch, m, weight, bias, act, slope, dtype)
-    y = torch.empty((m, weight.n), dtype=dtype, device=x.device)
-    d = _desc(0, 0, weight, bias, act, slope, y, m)
-    x_dtype = _DTYPES[x.dtype]
-    n = _workspace_bytes(m, weight.n, weight.k, _DTYPES[dtype], x_dtype)
-    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    rc = _lib.lib().y5_linear_i8(C.byref(d), x.data_ptr(), pitch, x_dtype, None if ws is None else ws.data_ptr(), n, _lib.raw_stream(x.device.index))
-    if rc:
-        _lib.check(rc)
-    return y
 
 
 def _check(name, x, weight, bias, act, dtype):
@@ -252,7 +189,9 @@ def linear_i8(x, weight, bias=None, act=None, slope=0.1, dtype=None):
     if k != weight.k:
         raise ValueError('rows of %d values, weights for %d' % (k, weight.k))
     if rows:
-        return _product(x, weight, bias, act, slope, dtype)
+        if not x.q.is_cuda or x.q.shape[0] == 0:
+            return _plain_product(x, weight, bias, act, slope, dtype).reshape(*x.lead, weight.n)
+        return _lib.calls().product(x.q, x.scale, weight.q, weight.scale, k, bias, _ACTS[act], slope, dtype, (*x.lead, weight.n))
     if x.dtype not in _DTYPES:
         raise TypeError('linear_i8 expects fp16, bf16, fp32 or Int8Rows, got %s' % x.dtype)
     if x.requires_grad:
@@ -260,8 +199,7 @@ def linear_i8(x, weight, bias=None, act=None, slope=0.1, dtype=None):
     if not x.is_cuda or x.numel() == 0:
         return _plain_product(quantize_rows(x), weight, bias, act, slope, dtype).reshape(*x.shape[:-1], weight.n)
     r, pitch = _rows_of(x)
-    y = _linear(r, pitch, r.shape[0], weight, bias, act, slope, dtype)
-    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], weight.n)
+    return _lib.calls().linear(r, pitch, r.shape[0], weight.q, weight.scale, k, bias, _ACTS[act], slope, dtype, (*x.shape[:-1], weight.n))
 
 
 def conv1x1_i8(x, weight, bias=None, act=None, slope=0.1, dtype=None):
@@ -285,8 +223,9 @@ def conv1x1_i8(x, weight, bias=None, act=None, slope=0.1, dtype=None):
     if x.shape[1] != weight.k:
         raise ValueError('%d channels, weights for %d' % (x.shape[1], weight.k))
     _refuse_grad('conv1x1_i8', x)
-    y = _linear(x, pitch, x.numel() // weight.k, weight, bias, act, slope, dtype)
-    return y.reshape(x.shape[0], *x.shape[2:], weight.n).movedim(-1, 1)
+    y = _lib.calls().linear(x, pitch, x.numel() // weight.k, weight.q, weight.scale, weight.k, bias, _ACTS[act], slope, dtype,
+                            (x.shape[0], *x.shape[2:], weight.n))
+    return y.movedim(-1, 1)
 
 
 class Int8Linear(nn.Module):
