@@ -277,3 +277,27 @@ def test_empty_and_module(dev):
         y.backward(torch.ones_like(y))
     ref = GroupNormRef(x, 4, None, None, 1e-5, 'leaky', dy=torch.ones(x.shape))
     close(m.weight.grad, ref.dgamma, ref.err_dgamma + 0.9 * (ref.z.abs() < 1e-5).sum((0, 2, 3)) * 1e-5, 'dgamma')
+
+
+def test_capture_beside_a_live_graph_is_refused(dev):
+    """A leaf whose accumulation node lives on the default stream cannot be reached by a captured gradient; the same leaf can once that graph
+    is gone."""
+    x, w, b, dy = (v.to(dev) for v in make((2, 16, 5, 4), F16, 47))
+    with torch.enable_grad():
+        leaves = [v.detach().clone().requires_grad_() for v in (x, w, b)]
+        alive = group_norm(leaves[0], 4, leaves[1], leaves[2], act='silu')
+        want = torch.autograd.grad(alive, leaves, dy, retain_graph=True)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            with pytest.raises(RuntimeError, match='live graph'):
+                group_norm(leaves[0], 4, leaves[1], leaves[2], act='silu')
+            with torch.no_grad():
+                group_norm(leaves[0], 4, leaves[1], leaves[2], act='silu')
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = torch.autograd.grad(group_norm(leaves[0], 4, leaves[1], leaves[2], act='silu'), leaves, dy)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(got, want))

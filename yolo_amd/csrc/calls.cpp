@@ -3,8 +3,10 @@
 // microseconds; the same steps in Python take ten (and sixty for the gradient, whose thread has to wait for the interpreter).
 // Arguments arrive checked (yolo_amd/groupnorm.py, yolo_amd/int8.py).
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -101,6 +103,17 @@ Tensor run_forward(const Tensor& x, const Norm& n, const Tensor& weight, const T
     return y;
 }
 
+// torch keeps one accumulation node a leaf as long as any graph of it lives, on the stream of the first.  The default stream cannot
+// join a capture: the captured gradient of a leaf whose node lives there ends the process, so its forward pass is refused.
+void check_leaf(const Tensor& t, const char* name) {
+    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node) return;
+    const auto stream = node->stream();
+    TORCH_CHECK(!stream || stream->id() != c10::hip::getDefaultHIPStream(t.get_device()).id(), "group_norm: ", name,
+                " has a live graph on the default stream, which its captured gradient would have to wait for: drop that graph before the capture");
+}
+
 struct GroupNorm : torch::autograd::Function<GroupNorm> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, Maybe weight, Maybe bias, int64_t pitch, int64_t groups, double eps,
                           int64_t act, double slope) {
@@ -155,8 +168,14 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
 
 Tensor group_norm(const Tensor& x, int64_t pitch, int64_t groups, Maybe weight, Maybe bias, double eps, int64_t act, double slope) {
     const Tensor w = or_none(weight), b = or_none(bias);
-    if (at::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad())))
+    if (at::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()))) {
+        if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
+            check_leaf(x, "x");
+            check_leaf(w, "weight");
+            check_leaf(b, "bias");
+        }
         return GroupNorm::apply(x, weight, bias, pitch, groups, eps, act, slope);
+    }
     return run_forward(x, Norm{pitch, groups, act, eps, slope}, w, b, Tensor());
 }
 

@@ -17,6 +17,9 @@ namespace {
 // wait for copies is a counted s_waitcnt vmcnt(N) that leaves the youngest half-tiles in flight.  128-byte LDS rows are
 // XOR-swizzled through the copies' source addresses.  Rows and bytes past the matrices fail the descriptors' range check and
 // arrive as zeros; descriptors start at the tile, so the matrices may be of any size.
+// Measured: 16384 x 4096 x 4096 in 209 us alone (2.63 POP/s; 214 behind its quantisation), the 8-bit library product of the same sizes
+// 267.  Bound by the clock that the matrix units' load leaves: a K-tile of 256 x 256 takes 1.4 us with every unit busy, its matrix
+// instructions alone 0.85 at 2.4 GHz.  12800 x 1024 x 512: 13 us, one round of 200 tiles whose eight K-tiles take 7 of them.
 // Hazards.  RAW: a half-tile is read no earlier than the phase after the counted wait that retired it, behind a barrier every
 // wave has passed after its own wait.  WAR: a slot is refilled one phase after its last read, and every phase drains its reads
 // (lgkmcnt(0)) before its first barrier.

@@ -9,10 +9,15 @@
 // HBM.  Every output needs sums over the whole image, which leaves two forms:
 //   resident  one workgroup owns a slice of whole groups of one image and keeps its values in registers between the sums and
 //             the normalisation: every value is read once and written once, one launch.  For slices of up to 16 vectors a
-//             thread.
+//             thread.  20 x 20 x 512 fp16 in 32 groups: 7 us, latency of one chain (load, sums, squares, store);
+//             4 x 40 x 40 x 256 fp32: 10 us (1.3 TB/s; 128 workgroups), its gradient 12.8.
 //   split     a statistics pass over chunks of every image, then a pass that merges the chunks' statistics and normalises.
 //             The second pass walks the images in the opposite order, so that what the first one read last is still in the
-//             256 MB cache in front of HBM.
+//             256 MB cache in front of HBM.  32 x 160 x 160 x 64 fp16 with silu: 30 us (3.5 TB/s; the values come from HBM) and
+//             40 us (5.3 TB/s, read from that cache and written); 32 x 80 x 80 x 256 bf16: 28 and 36, the gradient 43 (4.9 TB/s)
+//             and 54 (5.8 TB/s).  A copy reaches 5.2 TB/s from HBM, 7.1 from the cache.
+// One kernel for large maps would save the second read, but its workgroups would have to wait for each other, which two such
+// kernels on two streams can turn into a wait for ever.
 // The sums are taken in a fixed order (no atomics): the same call gives the same bits.
 #include "y5_common.h"
 
@@ -267,7 +272,8 @@ __global__ __launch_bounds__(R > 8 ? 1024 : R > 4 ? 512 : 256, 4) void gn_reside
 
 // ------------------------------------------------------------------------------------------ forward, split
 
-// grid (chunks, batch): (mean, M2) of every group over the chunk.  A thread sums differences from the first value it reads (K):
+// grid (chunks, batch): (mean, M2) of every group over the chunk.  Bound by HBM; four loads of 16 bytes in flight a thread and 6 to 8
+// waves a SIMD hide its latency.  A thread sums differences from the first value it reads (K):
 // where a map's mean is many deviations from zero, sum and sum of squares of the raw values would cancel.  The threads' means and
 // squares then meet as differences from one thread's mean of each group.
 template <typename T, int M>
@@ -363,7 +369,8 @@ __global__ __launch_bounds__(1024, sizeof(T) == 4 || M == kUniform ? 8 : 6) void
     });
 }
 
-// grid (runs of rows, batch), walked from the end.  A thread's first rows are on their way while the chunks' statistics are merged.
+// grid (runs of rows, batch), walked from the end.  Bound by the cache's reads and HBM's writes, with silu almost as much by the vector
+// units (busy for 23 of the 40 us that 52 million values take; the gradient below: 35 of 54).  A thread's first rows are on their way while the chunks' statistics are merged.
 template <typename T, int M, bool SILU>
 __global__ __launch_bounds__(1024, 6) void gn_apply_kernel(const GnArgs a, int run_rows) {
     constexpr int V = NormElem<T>::V, NG = M ? V : 1, U = 4;
@@ -480,7 +487,8 @@ __device__ __forceinline__ void grad_sums(const GnArgs& a, const float* tot, int
                });
 }
 
-// grid: slices * batch; LDS: part[blockDim.x * 2 V], tot[cols * 2 V], gs[2 * groups of the slice]
+// Gradient of a resident slice: x and dy stay in registers, xh and dz are computed twice from them (cheaper than the registers they would
+// take).  grid: slices * batch; LDS: part[blockDim.x * 2 V], tot[cols * 2 V], gs[2 * groups of the slice]
 template <typename T, int M, bool SILU, int R>
 __global__ __launch_bounds__(R > 4 ? 512 : 256, R > 4 && sizeof(T) == 2 ? 3 : 4) void gn_bwd_resident_kernel(const GnArgs a, const FastDiv by_cols, int slices) {
     constexpr int V = NormElem<T>::V, NG = M ? V : 1;
@@ -541,6 +549,7 @@ __global__ __launch_bounds__(R > 4 ? 512 : 256, R > 4 && sizeof(T) == 2 ? 3 : 4)
         }
 }
 
+// S1, S2 and the channels' sums of a chunk: x and dy read once, bound by HBM (210 MB: 43 us, 4.9 TB/s).
 // grid (chunks, batch); LDS as above for all groups
 template <typename T, int M, bool SILU>
 __global__ __launch_bounds__(1024, M == kUniform || sizeof(T) == 4 ? 5 : 4) void gn_bwd_stats_kernel(const GnArgs a) {
@@ -593,7 +602,7 @@ __global__ __launch_bounds__(1024, M == kUniform || sizeof(T) == 4 ? 5 : 4) void
     for (int g = t; g < s.groups; g += TB) a.part[at * s.groups + g] = make_float2(gs[2 * g], gs[2 * g + 1]);
 }
 
-// dbeta_c and dgamma_c: the rows of cpart ([rows][2][c]) added up, 16 of the 2 c columns by T threads.  red: T floats of LDS.
+// dbeta_c and dgamma_c, in a fixed order (4 us as a launch of its own, of which 2 are the launch): the rows of cpart ([rows][2][c]) added up, 16 of the 2 c columns by T threads.  red: T floats of LDS.
 __device__ __forceinline__ void sum_params(const float* __restrict__ cpart, int rows, int c, int dt, void* dweight, void* dbias, int block, float* red) {
     const int T = blockDim.x / 16 * 16, t = threadIdx.x;
     const int lc = t & 15, q = t >> 4, Q = T >> 4;

@@ -4,8 +4,9 @@
 // the scale NaN and zeros, so that everything computed from it is NaN.
 //
 // Memory bound: a value is read once, and written as one byte.  A row lives in the registers of the lanes that read it, so the
-// maximum is a few shuffles; with the group norm the normalised value is rounded once, to 8 bits, and no 16-bit tensor in between
-// is written or read.
+// maximum is a few moves between lanes; with the group norm the normalised value is rounded once, to 8 bits, and no 16-bit tensor in between
+// is written or read.  12800 x 1024 fp16: 9.5 us, 16384 x 4096 bf16: 37 us (5.4 TB/s); after a group norm 204800 x 256 with silu: 41
+// us for 157 MB (3.8 TB/s), bound by the vector units (busy for 33 of them), behind the 30 us of gn_stats_kernel.
 #include "y5_common.h"
 
 namespace {
@@ -93,8 +94,8 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsArgs a) {
             b0[i] = c < s.c ? ld_param(a.bias, c, s.param_dtype, 0.f) : 0.f;
         }
         norm_merge_chunks(s, a.part, b, red, gmean, grstd);
-        // mean and beta in one number: what that costs (the mean's magnitude over a deviation, times 2^-24) is far below the
-        // 2^-8 of the rounding that follows
+        // mean and beta in one number: that rounds as coarsely as holding the mean in 32 bits does (its magnitude over a
+        // deviation, times 2^-24), and is far below the 2^-8 of the rounding that follows wherever that mean is
         for (int c = t; c < a.q_ld; c += TB) {
             float ca = 0.f, cb = 0.f;
             if (c < s.c) {
