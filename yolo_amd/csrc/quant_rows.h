@@ -9,7 +9,10 @@ __device__ __forceinline__ float row_scale(unsigned bits, float* a) {
     const float m = __uint_as_float(bits);
     *a = m >= kZeroRow ? m : 0.f;
     if (bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
-    return *a / 127.f;
+    // a / 127 to nearest: quotient by the rounded reciprocal, its exact remainder, one step (that is what a division does, without the
+    // cases it also has to cover; equal to it for every value from 2^-120 up)
+    const float y = 1.f / 127.f, q = *a * y;
+    return __builtin_fmaf(__builtin_fmaf(-q, 127.f, *a), y, q);
 }
 
 // The whole number nearest to v * 127 / a, as the low byte of a word (the rest of the word is not zero).  Adding 1.5 * 2^23 (2^52)

@@ -60,8 +60,13 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsArgs a) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) off[v] = (v * a.lanes + l) * V;
     norm_u32x4 raw[NV];  // the values as they are in memory
+    // the row to load next and the row to store next, moved along by additions: 64-bit products of row and pitch would cost a tenth of
+    // all that a row of 256 values takes
+    const T* xr = static_cast<const T*>(a.x) + (base + row0 + sub) * a.x_ld;
+    signed char* qr = a.q + (size_t)(base + row0 + sub) * a.q_ld;
+    float* sr = a.scale + base + row0 + sub;
+    const long long x_step = step * a.x_ld, q_step = (long long)step * a.q_ld;
     auto load = [&](long long row) {
-        const T* xr = static_cast<const T*>(a.x) + (base + row) * a.x_ld;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int n = row < row1 ? a.k - off[v] : 0;
@@ -72,6 +77,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsArgs a) {
                 raw[v] = __builtin_bit_cast(norm_u32x4, u);
             }
         }
+        xr += x_step;
     };
     auto unpack = [&](int v) {  // the empty statement keeps the compiler from holding the values unpacked
         asm volatile("" : "+v"(raw[v]));
@@ -149,18 +155,24 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsArgs a) {
         typename InvOf<T, NORM != kPlain>::type inv;
         inv.set(m, top < 0x7f800000u);
         if (row < row1) {
-            signed char* qr = a.q + (size_t)(base + row) * a.q_ld;
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 if (off[v] >= a.q_ld) continue;
                 unsigned w[V];
-                const NormArr<T> x = unpack(v);
+                if constexpr (NORM != kPlain) {  // raw holds the next row: not touched here, or its loads would be waited for
 #pragma unroll
-                for (int e = 0; e < V; ++e) w[e] = inv(NORM != kPlain ? z[NORM != kPlain ? v : 0][e] : (float)x.v[e]);
+                    for (int e = 0; e < V; ++e) w[e] = inv(z[v][e]);
+                } else {
+                    const NormArr<T> x = unpack(v);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) w[e] = inv((float)x.v[e]);
+                }
                 st_bytes<V>(qr + off[v], w, top < 0x7f800000u);
             }
-            if (l == 0) a.scale[base + row] = scale;
+            if (l == 0) *sr = scale;
         }
+        qr += q_step;
+        sr += step;
     }
 }
 
