@@ -301,3 +301,31 @@ def test_capture_beside_a_live_graph_is_refused(dev):
             graph.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize('shape,groups,reps,dtype', [((3, 64, 160, 160), 32, 16, F16), ((3, 256, 20, 20), 32, 22, F16), ((3, 256, 20, 20), 32, 171, BF16), ((3, 512, 10, 10), 32, 40, F32),
+                                                     ((3, 75, 27, 27), 25, 667, BF16), ((3, 256, 40, 40), 32, 22, F16), ((3, 128, 40, 40), 32, 11, BF16)],
+                         ids=lambda v: str(v).replace(' ', ''))
+def test_large_batches(dev, shape, groups, reps, dtype):
+    """Batches that take wide slices, more vectors a thread, the split form for a gradient alone, or stores past the cache: three images over and
+    over, whose results are as right as those of the three and the same every time.  The parameters' gradients add up to 2001 rows in 16
+    chains, of 126 + 16 additions: (142 + 64) / 64 times the bound of the three."""
+    x, w, b, dy = make(shape, dtype, sum(shape), F32)
+    ref = GroupNormRef(x, groups, w, b, 1e-5, 'silu', dy=dy)
+
+    def over(v):
+        v = v.to(dev).movedim(1, -1).contiguous()
+        return v.repeat(reps, *[1] * (v.dim() - 1)).movedim(-1, 1)
+
+    with torch.enable_grad():
+        leaves = [v.requires_grad_() for v in (over(x), w.to(dev), b.to(dev))]
+        y = group_norm(leaves[0], groups, leaves[1], leaves[2], act='silu')
+        dx, dw, db = torch.autograd.grad(y, leaves, over(dy))
+    y = y.detach()
+    inference = group_norm(leaves[0].detach(), groups, leaves[1].detach(), leaves[2].detach(), act='silu')
+    for got, want, err, name in ((y, ref.y, ref.err_y, 'y'), (dx, ref.dx, ref.err_dx, 'dx'), (inference, ref.y, ref.err_y, 'y without gradient')):
+        close(got[-3:], want, err, name)
+        for i in range(reps):
+            assert torch.equal(got[3 * i:3 * i + 3], got[-3:]), (name, i)
+    close(dw, reps * ref.dgamma, 4 * reps * ref.err_dgamma, 'dgamma')
+    close(db, reps * ref.dbeta, 4 * reps * ref.err_dbeta, 'dbeta')

@@ -13,9 +13,10 @@
 //             4 x 40 x 40 x 256 fp32: 10 us (1.3 TB/s; 128 workgroups), its gradient 12.8.
 //   split     a statistics pass over chunks of every image, then a pass that merges the chunks' statistics and normalises.
 //             The second pass walks the images in the opposite order, so that what the first one read last is still in the
-//             256 MB cache in front of HBM.  32 x 160 x 160 x 64 fp16 with silu: 30 us (3.5 TB/s; the values come from HBM) and
-//             40 us (5.3 TB/s, read from that cache and written); 32 x 80 x 80 x 256 bf16: 28 and 36, the gradient 43 (4.9 TB/s)
-//             and 54 (5.8 TB/s).  A copy reaches 5.2 TB/s from HBM, 7.1 from the cache.
+//             256 MB cache in front of HBM.  32 x 160 x 160 x 64 fp16 with silu: 30 us (105 MB from HBM, while the last call's result
+//             is written back; 23 behind nothing of the kind) and 40 us (5.3 TB/s, read from that cache and written);
+//             32 x 80 x 80 x 256 bf16 for training: 21 (5.1 TB/s) and 37, the gradient 40 (5.3 TB/s) and 51 (6.2 TB/s).  A copy
+//             reaches 5.2 TB/s from HBM, 7.1 from the cache.
 // One kernel for large maps would save the second read, but its workgroups would have to wait for each other, which two such
 // kernels on two streams can turn into a wait for ever.
 // The sums are taken in a fixed order (no atomics): the same call gives the same bits.
@@ -35,6 +36,7 @@ struct GnArgs {
     float* cpart;        // backward: [batch * chunks][2][c], a chunk's sums of dz and of dz * xh
     long long x_row, y_row, dy_row, dx_row;  // pitch of a virtual row, in elements
     long long x_img, y_img, dy_img, dx_img;  // of an image
+    int past;  // y or dx is stored past the cache in front of HBM
 };
 
 // tot[j * N + i] = sum of v[i] over the threads of column j, in a fixed order.  part: blockDim.x * N floats of LDS.
@@ -173,9 +175,16 @@ __device__ __forceinline__ NormArr<T> unpack(Raw& r) {
     return __builtin_bit_cast(NormArr<T>, r);
 }
 template <typename T, int M>
-__device__ __forceinline__ void st_col(T* p, int nv, const Raw& r) {
-    if (M != kCut || nv >= NormElem<T>::V) reinterpret_cast<NormVec<T>*>(p)->v = r;
-    else st_part(p, nv, __builtin_bit_cast(NormArr<T>, r).v);
+__device__ __forceinline__ void st_col(T* p, int nv, const Raw& r, int past) {
+    if (M != kCut || nv >= NormElem<T>::V) {
+        if (past) {
+            asm volatile("" ::: "memory");  // keeps the compiler from making one store of the two
+            __builtin_nontemporal_store(r, &reinterpret_cast<NormVec<T>*>(p)->v);
+            asm volatile("" ::: "memory");
+        } else {
+            reinterpret_cast<NormVec<T>*>(p)->v = r;
+        }
+    } else st_part(p, nv, __builtin_bit_cast(NormArr<T>, r).v);
 }
 
 // z = act(gamma (x - mean) rstd + beta) of one vector, rounded once
@@ -267,7 +276,7 @@ __global__ __launch_bounds__(R > 8 ? 1024 : R > 4 ? 512 : 256, 4) void gn_reside
     T* yb = static_cast<T*>(a.y) + (size_t)b * a.y_img + col.off;
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (const int nv = valid(i)) st_col<T, M>(yb + (size_t)(r + i * RT) * a.y_row, nv, normalise<T, SILU, NG>(raw[i], mean, A, B, s.slope));
+        if (const int nv = valid(i)) st_col<T, M>(yb + (size_t)(r + i * RT) * a.y_row, nv, normalise<T, SILU, NG>(raw[i], mean, A, B, s.slope), a.past);
 }
 
 // ------------------------------------------------------------------------------------------ forward, split
@@ -370,7 +379,7 @@ __global__ __launch_bounds__(1024, sizeof(T) == 4 || M == kUniform ? 8 : 6) void
 }
 
 // grid (runs of rows, batch), walked from the end.  Bound by the cache's reads and HBM's writes, with silu almost as much by the vector
-// units (busy for 23 of the 40 us that 52 million values take; the gradient below: 35 of 54).  A thread's first rows are on their way while the chunks' statistics are merged.
+// units (busy for 23 of the 40 us that 52 million values take; the gradient below: 35 of 51).  A thread's first rows are on their way while the chunks' statistics are merged.
 template <typename T, int M, bool SILU>
 __global__ __launch_bounds__(1024, 6) void gn_apply_kernel(const GnArgs a, int run_rows) {
     constexpr int V = NormElem<T>::V, NG = M ? V : 1, U = 4;
@@ -414,7 +423,7 @@ __global__ __launch_bounds__(1024, 6) void gn_apply_kernel(const GnArgs a, int r
         load(row + U * RT);
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (row + u * RT < row1) st_col<T, M>(yb + (size_t)(row + u * RT) * a.y_row, col.valid(s, row + u * RT), o[u]);
+            if (row + u * RT < row1) st_col<T, M>(yb + (size_t)(row + u * RT) * a.y_row, col.valid(s, row + u * RT), o[u], a.past);
     }
 }
 
@@ -490,7 +499,7 @@ __device__ __forceinline__ void grad_sums(const GnArgs& a, const float* tot, int
 // Gradient of a resident slice: x and dy stay in registers, xh and dz are computed twice from them (cheaper than the registers they would
 // take).  grid: slices * batch; LDS: part[blockDim.x * 2 V], tot[cols * 2 V], gs[2 * groups of the slice]
 template <typename T, int M, bool SILU, int R>
-__global__ __launch_bounds__(R > 4 ? 512 : 256, R > 4 && sizeof(T) == 2 ? 3 : 4) void gn_bwd_resident_kernel(const GnArgs a, const FastDiv by_cols, int slices) {
+__global__ __launch_bounds__(R > 2 ? 512 : 256, R > 4 && sizeof(T) == 2 ? 3 : 4) void gn_bwd_resident_kernel(const GnArgs a, const FastDiv by_cols, int slices) {
     constexpr int V = NormElem<T>::V, NG = M ? V : 1;
     extern __shared__ float lds[];
     const NormShape& s = a.s;
@@ -545,11 +554,11 @@ __global__ __launch_bounds__(R > 4 ? 512 : 256, R > 4 && sizeof(T) == 2 ? 3 : 4)
         if (const int nv = valid(i)) {
             float xh[V], dz[V];
             col.template local<SILU>(rx[i], rd[i], xh, dz, s.slope);
-            st_col<T, M>(ob + (size_t)(r + i * RT) * a.dx_row, nv, col.grad(xh, dz, s1, s2));
+            st_col<T, M>(ob + (size_t)(r + i * RT) * a.dx_row, nv, col.grad(xh, dz, s1, s2), a.past);
         }
 }
 
-// S1, S2 and the channels' sums of a chunk: x and dy read once, bound by HBM (210 MB: 43 us, 4.9 TB/s).
+// S1, S2 and the channels' sums of a chunk: x and dy read once, bound by HBM (210 MB: 40 us, 5.3 TB/s).
 // grid (chunks, batch); LDS as above for all groups
 template <typename T, int M, bool SILU>
 __global__ __launch_bounds__(1024, M == kUniform || sizeof(T) == 4 ? 5 : 4) void gn_bwd_stats_kernel(const GnArgs a) {
@@ -704,7 +713,7 @@ __global__ __launch_bounds__(1024, M == kUniform || sizeof(T) == 4 ? 5 : 4) void
         load(row + U * RT);
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (row + u * RT < row1) st_col<T, M>(ob + (size_t)(row + u * RT) * a.dx_row, col.valid(s, row + u * RT), o[u]);
+            if (row + u * RT < row1) st_col<T, M>(ob + (size_t)(row + u * RT) * a.dx_row, col.valid(s, row + u * RT), o[u], a.past);
     }
 }
 
@@ -722,34 +731,65 @@ int run_rows(const NormShape& s, int esize) {
     return rows < 1 ? 1 : (int)rows;
 }
 
-constexpr int kResidentAlone = 32 << 10;  // bytes of a slice that few workgroups may hold all the same
+constexpr int kResidentAlone = 32 << 10;    // bytes of a slice that few workgroups may hold all the same
+constexpr long long kCache = 256 << 20;     // bytes of the cache in front of HBM
 
-// A resident slice: whole groups, and 64 bytes of a pixel (half a cache line, so that little is read twice) where that leaves a workgroup
-// for every compute unit.  False where no slice fits the registers, or where a few workgroups would work long while the chip idles.
+long long tensor_bytes(const NormShape& s, int esize) { return (long long)s.batch * s.pixels * s.c * esize; }
+
+// A resident slice: whole groups, and 128 bytes of a pixel - a cache line - or as much as leaves a workgroup for every compute unit (from
+// 64 bytes to 128, forward and gradient: 64 x 40 x 40 x 256 fp16 90 -> 83 us, 512 x 10 x 10 x 512 fp16 104 -> 86, fp32 171 -> 131).  False where
+// no slice fits the registers, or where a few workgroups would work long while the chip idles.
+// The gradient of 16-bit values has registers for four vectors of x and dy a thread; eight leave half the waves, which a narrower slice is
+// better than (32 x 20 x 20 x 512: 30 us against 32) and only in small calls the split form is not (32 x 40 x 40 x 128, 13 MB a tensor: 33 us
+// against 42 split; 128 x 20 x 20 x 256, 26 MB: 52 against 50).  Parts of lines are read and written twice, which costs little as long as the
+// cache holds the call (64 bytes of 26 MB: 47 us against 56 split; of 105 MB: 162 against 142).
 struct Resident {
     int cols, threads, r;
 };
-bool resident_of(const NormShape& s, int esize, const int (&cap)[3][2], Resident* out) {
-    const int V = 16 / esize;
-    int cols = s.cols;
-    if (s.k == 1) {
-        cols = s.cpg / norm_gcd(s.cpg, V);  // lcm(cpg, V) / V columns hold whole groups and whole vectors
-        while (cols * 16 < 64 && s.cols % (cols * 2) == 0 && (long long)s.batch * (s.cols / (cols * 2)) >= 256) cols *= 2;
-    }
-    const long long wgs = (long long)s.batch * (s.cols / cols), bytes = (long long)s.vrows * cols * 16;
-    if (bytes > kResidentAlone && wgs < 128) return false;
+constexpr int kFwdCap[][2] = {{256, 4}, {512, 8}, {1024, 16}};  // threads, vectors a thread
+constexpr int kBwdCap[][2] = {{256, 2}, {256, 4}, {512, 4}, {512, 8}};
+
+template <int N>
+bool resident_fit(const NormShape& s, int cols, const int (&cap)[N][2], Resident* out) {
     for (const auto& c : cap) {
-        const int threads = c[0], r = c[1];
-        if (cols > threads) continue;
-        if ((long long)(threads / cols) * r >= s.vrows) {
-            *out = {cols, threads, r};
+        if (cols <= c[0] && (long long)(c[0] / cols) * c[1] >= s.vrows) {
+            *out = {cols, c[0], c[1]};
             return true;
         }
     }
     return false;
 }
-constexpr int kFwdCap[3][2] = {{256, 4}, {512, 8}, {1024, 16}};
-constexpr int kBwdCap[3][2] = {{256, 2}, {256, 4}, {512, 8}};
+
+bool resident_of(const NormShape& s, int esize, bool bwd, Resident* out) {
+    const int V = 16 / esize;
+    const long long tensors = 3 * tensor_bytes(s, esize);
+    for (int width = 128; width >= 64; width /= 2) {
+        int cols = s.cols;
+        if (s.k == 1) {
+            cols = s.cpg / norm_gcd(s.cpg, V);  // lcm(cpg, V) / V columns hold whole groups and whole vectors
+            while (cols * 16 < width && s.cols % (cols * 2) == 0 && (long long)s.batch * (s.cols / (cols * 2)) >= 256) cols *= 2;
+        }
+        const long long wgs = (long long)s.batch * (s.cols / cols), bytes = (long long)s.vrows * cols * 16;
+        if (bytes > kResidentAlone && wgs < 128) return false;
+        if (!bwd) {
+            if (resident_fit(s, cols, kFwdCap, out)) return true;
+        } else if (resident_fit(s, cols, kBwdCap, out)) {
+            if (esize == 2 && out->r > 4 ? width == 64 && tensors <= 64 << 20 : cols * 16 >= 128 || tensors <= kCache) return true;
+        }
+    }
+    return false;
+}
+
+// What the caller has on hand beside the result is worth more in the cache than the result: a map that fills it with dirty lines makes the
+// next kernels wait for those to be written (the statistics of 105 MB take 23 us where the cache holds clean lines, 30 after such a map, 42
+// after twice of it).  The result goes past the cache where x and y - for training x, y or dx, and dy - do not fit it together: 210 MB norm
+// and 1 x 1 convolution in turn 372 -> 351 us, forward and gradient 323 -> 276 (105 MB: 155 -> 146).  Where they fit, what reads the result
+// next pays more than is gained (norm and convolution of 105 MB: 104 -> 107 us, 79 MB: 81 -> 82).
+// Not for resident slices of an image, whose parts of lines meet in the cache (64 bytes of 157 MB: 110 -> 120 us with a pass over the result
+// behind it; 128 bytes of 157 MB: 101 -> 111); for whole images (219 MB of 75 channels) 257 -> 245.
+int past_cache(const NormShape& s, int esize, int tensors, const Resident* res) {
+    return (!res || res->cols == s.cols) && tensors * tensor_bytes(s, esize) > kCache;
+}
 
 GnArgs make_args(const y5_group_norm_desc& d, const NormShape& s) {
     GnArgs a{};
@@ -890,7 +930,7 @@ int y5_group_norm_work(const y5_group_norm_desc& d, int what, size_t* bytes) {
     if (rc) return rc;
     Resident r;
     const int es = norm_elem_size(d.dtype);
-    const bool res = what == Y5_GN_BACKWARD ? resident_of(s, es, kBwdCap, &r) : what == Y5_GN_FORWARD && resident_of(s, es, kFwdCap, &r);
+    const bool res = what != Y5_GN_ROWS && resident_of(s, es, what == Y5_GN_BACKWARD, &r);
     *bytes = work_of(s, res, what == Y5_GN_BACKWARD).total;
     return Y5_OK;
 }
@@ -903,11 +943,12 @@ int y5_launch_group_norm(const y5_group_norm_desc& d, hipStream_t st) {
     Y5_REQUIRE(!d.mean == !d.rstd, "group_norm: mean and rstd go together");
     const int es = norm_elem_size(d.dtype);
     Resident r;
-    const bool res = resident_of(s, es, kFwdCap, &r);
+    const bool res = resident_of(s, es, false, &r);
     const GnWork w = work_of(s, res, false);
     if (w.total && (!d.workspace || d.workspace_bytes < w.total)) return y5_fail(Y5_EWORKSPACE, "group_norm: workspace of %zu bytes, %zu needed", d.workspace ? d.workspace_bytes : (size_t)0, w.total);
     Y5_REQUIRE(!w.total || y5_aligned16(d.workspace), "group_norm: misaligned workspace");
     GnArgs a = make_args(d, s);
+    a.past = past_cache(s, es, d.mean ? 3 : 2, res ? &r : nullptr);
     a.part = static_cast<float2*>(d.workspace);
     return GN_DISPATCH(forward_act, d.dtype, mode_of(s, es), a, res ? &r : nullptr, st);
 }
@@ -920,11 +961,12 @@ int y5_launch_group_norm_bwd(const y5_group_norm_desc& d, hipStream_t st) {
     Y5_REQUIRE(d.mean && d.rstd, "group_norm_backward: null mean or rstd");
     const int es = norm_elem_size(d.dtype);
     Resident r;
-    const bool res = resident_of(s, es, kBwdCap, &r);
+    const bool res = resident_of(s, es, true, &r);
     const GnWork w = work_of(s, res, true);
     if (!d.workspace || d.workspace_bytes < w.total) return y5_fail(Y5_EWORKSPACE, "group_norm_backward: workspace of %zu bytes, %zu needed", d.workspace ? d.workspace_bytes : (size_t)0, w.total);
     Y5_REQUIRE(y5_aligned16(d.workspace), "group_norm_backward: misaligned workspace");
     GnArgs a = make_args(d, s);
+    a.past = past_cache(s, es, 3, res ? &r : nullptr);
     a.part = static_cast<float2*>(d.workspace);
     a.cpart = reinterpret_cast<float*>(static_cast<char*>(d.workspace) + w.part);
     return GN_DISPATCH(backward_act, d.dtype, mode_of(s, es), a, res ? &r : nullptr, st);
