@@ -27,13 +27,18 @@ __device__ __forceinline__ void ld_vec(const T* p, T (&v)[NormElem<T>::V]) {
 #pragma unroll
     for (int e = 0; e < NormElem<T>::V; ++e) v[e] = u.v[e];
 }
-// the first n elements, zeros behind them; nothing behind the n-th is touched
+// the first n elements, zeros behind them; nothing behind the n-th is touched: the first is read in its place, so that all are on their way
+// at once (a branch an element waits for each)
 template <typename T>
 __device__ __forceinline__ void ld_part(const T* p, int n, T (&v)[NormElem<T>::V]) {
 #pragma unroll
-    for (int e = 0; e < NormElem<T>::V; ++e) {
-        v[e] = (T)0.f;
-        if (e < n) v[e] = p[e];
+    for (int e = 0; e < NormElem<T>::V; ++e) v[e] = (T)0.f;
+    if (n > 0) {
+#pragma unroll
+        for (int e = 0; e < NormElem<T>::V; ++e) {
+            const T x = p[e < n ? e : 0];
+            v[e] = e < n ? x : (T)0.f;
+        }
     }
 }
 template <typename T>

@@ -76,6 +76,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsArgs a) {
                 NormArr<T> u;
                 ld_part(xr + off[v], n, u.v);
                 raw[v] = __builtin_bit_cast(norm_u32x4, u);
+                asm volatile("" : "+v"(raw[v]));  // packed here: the elements would take their registers through the whole loop
             }
         }
         xr += x_step;
