@@ -673,15 +673,13 @@ __global__ __launch_bounds__(1024, M == kUniform || sizeof(T) == 4 ? 5 : 4) void
     const float2* pb = a.part + (size_t)b * s.chunks * s.groups;
     for (int g0 = 0; g0 < s.groups; g0 += TB) {  // S1 / n and S2 / n of every group: the chunks' sums added up
         const int G = s.groups - g0 < TB ? s.groups - g0 : TB;
-        const int S = TB / G, g = t % G, q = t / G;
+        const int S = norm_merge_threads(s, TB, G), g = t % G, q = t / G;
         float s1 = 0.f, s2 = 0.f;
         if (q < S) {
-#pragma unroll 8
-            for (int i = q; i < s.chunks; i += S) {
-                const float2 m = pb[(size_t)i * s.groups + g0 + g];
+            norm_each_chunk(s, pb + g0 + g, q, S, [&](int, float2 m) {
                 s1 += m.x;
                 s2 += m.y;
-            }
+            });
             red[2 * t] = s1;
             red[2 * t + 1] = s2;
         }

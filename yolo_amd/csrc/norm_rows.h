@@ -139,6 +139,29 @@ struct NormShape {
     FastDiv by_c, by_cpg, by_cols;
 };
 
+// Merging the chunks of a group: norm_merge_threads() of T threads for G groups share it, each adds up four chunks or more, four of them on
+// their way at a time, and one of the threads the others' sums, one after the other (with every thread of few groups that alone
+// took 9 us)
+__device__ __forceinline__ int norm_merge_threads(const NormShape& s, int T, int G) {
+    const int all = T / G, most = (s.chunks + 3) / 4;
+    return all < most ? all : most;
+}
+// f(chunk, what it left) for thread r of S; p: what the group's first chunk left
+template <typename F>
+__device__ __forceinline__ void norm_each_chunk(const NormShape& s, const float2* __restrict__ p, int r, int S, F f) {
+    for (int i = r; i < s.chunks; i += 4 * S) {
+        float2 m[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int k = i + u * S < s.chunks ? i + u * S : i;
+            m[u] = p[(size_t)k * s.groups];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (i + u * S < s.chunks) f(i + u * S, m[u]);
+    }
+}
+
 // pixels of chunk i of an image
 __device__ __forceinline__ int norm_chunk_pixels(const NormShape& s, int i) {
     const long long p0 = (long long)i * s.chunk_rows * s.k, p1 = p0 + (long long)s.chunk_rows * s.k;
@@ -156,19 +179,17 @@ __device__ __forceinline__ void norm_merge_chunks(const NormShape& s, const floa
     const float npix = (float)s.cpg;
     for (int g0 = 0; g0 < s.groups; g0 += T) {
         const int G = s.groups - g0 < T ? s.groups - g0 : T;
-        const int S = T / G;  // threads of a group
+        const int S = norm_merge_threads(s, T, G);
         const int g = t % G, r = t / G;
         float s1 = 0.f, s2 = 0.f, K = 0.f;
         if (r < S) {
             K = pb[g0 + g].x;
-#pragma unroll 8
-            for (int i = r; i < s.chunks; i += S) {
-                const float2 m = pb[(size_t)i * s.groups + g0 + g];
+            norm_each_chunk(s, pb + g0 + g, r, S, [&](int i, float2 m) {
                 const float n = (float)norm_chunk_pixels(s, i) * npix;
                 const float d = m.x - K;
                 s1 = __builtin_fmaf(n, d, s1);
                 s2 += __builtin_fmaf(n * d, d, m.y);
-            }
+            });
             red[2 * t] = s1;
             red[2 * t + 1] = s2;
         }
