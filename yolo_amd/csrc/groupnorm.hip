@@ -159,6 +159,28 @@ struct Column {
     }
 };
 
+// The rows of a resident slice that a thread holds: r, r + RT, ... below `limit` as whole vectors, and `tail` elements of the last row
+// where that is cut short within the thread's vector.  One piece of code for the one vector that may be cut: in every turn of the
+// unrolled loops it would be most of the kernel, and a small map's time is that of fetching it.
+template <typename T, int M>
+struct Held {
+    bool active;
+    int limit, tail;
+    __device__ __forceinline__ void init(const NormShape& s, const Column<T, M>& col, int r, int RT) {
+        active = r < RT;
+        limit = s.vrows;
+        tail = 0;
+        if constexpr (M == kCut) {
+            const int last = s.vrows - 1, nv = col.valid(s, last);
+            if (nv < NormElem<T>::V) {
+                limit = last;
+                if (active && last % RT == r) tail = nv;
+            }
+        }
+    }
+    __device__ __forceinline__ bool has(int row) const { return active && row < limit; }
+};
+
 // A vector of T as the 16 bytes it is in memory: what is kept across a barrier stays packed.
 typedef norm_u32x4 Raw;
 template <typename T, int M>
@@ -224,12 +246,13 @@ __global__ __launch_bounds__(R > 8 ? 1024 : R > 4 ? 512 : 256, 4) void gn_reside
     const int gn = M ? s.cpg : s.cpg / V;                        // entries of a group in tot
     const T* xb = static_cast<const T*>(a.x) + (size_t)b * a.x_img + col.off;
     Raw raw[R];
-    auto valid = [&](int i) { return active && r + i * RT < s.vrows ? col.valid(s, r + i * RT) : 0; };
+    Held<T, M> held;
+    held.init(s, col, r, RT);
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int nv = valid(i);
-        if (nv) raw[i] = ld_col<T, M>(xb + (size_t)(r + i * RT) * a.x_row, nv);
-    }
+    for (int i = 0; i < R; ++i)
+        if (held.has(r + i * RT)) raw[i] = ld_col<T, M>(xb + (size_t)(r + i * RT) * a.x_row, V);
+    Raw cut = {0, 0, 0, 0};
+    if (held.tail) cut = ld_col<T, M>(xb + (size_t)held.limit * a.x_row, held.tail);
     float A[V], B[V];  // gamma (times 1 / deviation, later) and beta: on their way with the values
     col.params(s, a.weight, 1.f, A);
     col.params(s, a.bias, 0.f, B);
@@ -238,11 +261,16 @@ __global__ __launch_bounds__(R > 8 ? 1024 : R > 4 ? 512 : 256, 4) void gn_reside
     for (int e = 0; e < NG; ++e) acc[e] = 0.f;
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (valid(i)) {
+        if (held.has(r + i * RT)) {
             const NormArr<T> x = unpack<T>(raw[i]);
 #pragma unroll
             for (int e = 0; e < V; ++e) acc[M ? e : 0] += (float)x.v[e];
         }
+    if constexpr (M == kCut) {
+        const NormArr<T> x = unpack<T>(cut);
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] += (float)x.v[e];
+    }
     const float inv_n = 1.f / ((float)s.pixels * (float)s.cpg);
     col_sum<NG>(acc, j, r, RT, cols, part, tot);
     group_sum2(G, gn, s.k, s.c, [&](int i) { return make_float2(tot[i], 0.f); }, [&](int g, float2 v) { gs[2 * g] = v.x * inv_n; });
@@ -254,14 +282,22 @@ __global__ __launch_bounds__(R > 8 ? 1024 : R > 4 ? 512 : 256, 4) void gn_reside
     }
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (const int nv = valid(i)) {
+        if (held.has(r + i * RT)) {
             const NormArr<T> x = unpack<T>(raw[i]);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const float d = (float)x.v[e] - mean[M ? e : 0];
-                if (M != kCut || e < nv) acc[M ? e : 0] = __builtin_fmaf(d, d, acc[M ? e : 0]);
+                acc[M ? e : 0] = __builtin_fmaf(d, d, acc[M ? e : 0]);
             }
         }
+    if constexpr (M == kCut) {
+        const NormArr<T> x = unpack<T>(cut);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float d = (float)x.v[e] - mean[e];
+            if (e < held.tail) acc[e] = __builtin_fmaf(d, d, acc[e]);
+        }
+    }
     col_sum<NG>(acc, j, r, RT, cols, part, tot);
     group_sum2(G, gn, s.k, s.c, [&](int i) { return make_float2(tot[i], 0.f); }, [&](int g, float2 v) { gs[2 * g + 1] = 1.f / sqrtf(v.x * inv_n + s.eps); });
     if (a.mean) {
@@ -276,7 +312,8 @@ __global__ __launch_bounds__(R > 8 ? 1024 : R > 4 ? 512 : 256, 4) void gn_reside
     T* yb = static_cast<T*>(a.y) + (size_t)b * a.y_img + col.off;
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (const int nv = valid(i)) st_col<T, M>(yb + (size_t)(r + i * RT) * a.y_row, nv, normalise<T, SILU, NG>(raw[i], mean, A, B, s.slope), a.past);
+        if (held.has(r + i * RT)) st_col<T, M>(yb + (size_t)(r + i * RT) * a.y_row, V, normalise<T, SILU, NG>(raw[i], mean, A, B, s.slope), a.past);
+    if (held.tail) st_col<T, M>(yb + (size_t)held.limit * a.y_row, held.tail, normalise<T, SILU, NG>(cut, mean, A, B, s.slope), a.past);
 }
 
 // ------------------------------------------------------------------------------------------ forward, split
@@ -499,7 +536,7 @@ __device__ __forceinline__ void grad_sums(const GnArgs& a, const float* tot, int
 // Gradient of a resident slice: x and dy stay in registers, xh and dz are computed twice from them (cheaper than the registers they would
 // take).  grid: slices * batch; LDS: part[blockDim.x * 2 V], tot[cols * 2 V], gs[2 * groups of the slice]
 template <typename T, int M, bool SILU, int R>
-__global__ __launch_bounds__(R > 2 ? 512 : 256, R > 4 && sizeof(T) == 2 ? 3 : 4) void gn_bwd_resident_kernel(const GnArgs a, const FastDiv by_cols, int slices) {
+__global__ __launch_bounds__(R > 2 ? 512 : 256, sizeof(T) == 2 && (R > 4 || M == kCut) ? 3 : 4) void gn_bwd_resident_kernel(const GnArgs a, const FastDiv by_cols, int slices) {
     constexpr int V = NormElem<T>::V, NG = M ? V : 1;
     extern __shared__ float lds[];
     const NormShape& s = a.s;
@@ -514,29 +551,44 @@ __global__ __launch_bounds__(R > 2 ? 512 : 256, R > 4 && sizeof(T) == 2 ? 3 : 4)
     const T* xb = static_cast<const T*>(a.x) + (size_t)b * a.x_img + col.off;
     const T* db = static_cast<const T*>(a.dy) + (size_t)b * a.dy_img + col.off;
     Raw rx[R], rd[R];
-    auto valid = [&](int i) { return active && r + i * RT < s.vrows ? col.valid(s, r + i * RT) : 0; };
+    Held<T, M> held;
+    held.init(s, col, r, RT);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        if (const int nv = valid(i)) {
-            rx[i] = ld_col<T, M>(xb + (size_t)(r + i * RT) * a.x_row, nv);
-            rd[i] = ld_col<T, M>(db + (size_t)(r + i * RT) * a.dy_row, nv);
+        if (held.has(r + i * RT)) {
+            rx[i] = ld_col<T, M>(xb + (size_t)(r + i * RT) * a.x_row, V);
+            rd[i] = ld_col<T, M>(db + (size_t)(r + i * RT) * a.dy_row, V);
         }
+    }
+    Raw cx = {0, 0, 0, 0}, cd = {0, 0, 0, 0};
+    if (held.tail) {
+        cx = ld_col<T, M>(xb + (size_t)held.limit * a.x_row, held.tail);
+        cd = ld_col<T, M>(db + (size_t)held.limit * a.dy_row, held.tail);
     }
     float acc[2 * V];
 #pragma unroll
     for (int e = 0; e < 2 * V; ++e) acc[e] = 0.f;
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (const int nv = valid(i)) {
+        if (held.has(r + i * RT)) {
             float xh[V], dz[V];
             col.template local<SILU>(rx[i], rd[i], xh, dz, s.slope);
 #pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (M != kCut || e < nv) {
-                    acc[e] += dz[e];
-                    acc[V + e] = __builtin_fmaf(dz[e], xh[e], acc[V + e]);
-                }
+            for (int e = 0; e < V; ++e) {
+                acc[e] += dz[e];
+                acc[V + e] = __builtin_fmaf(dz[e], xh[e], acc[V + e]);
+            }
         }
+    if (held.tail) {
+        float xh[V], dz[V];
+        col.template local<SILU>(cx, cd, xh, dz, s.slope);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (e < held.tail) {
+                acc[e] += dz[e];
+                acc[V + e] = __builtin_fmaf(dz[e], xh[e], acc[V + e]);
+            }
+    }
     col_sum<2 * V>(acc, j, r, RT, cols, part, tot);
     const int c0 = s.k > 1 ? 0 : slice * cols * V, channels = s.k > 1 ? s.c : cols * V;
     const int g0 = (int)fdiv(c0, s.by_cpg), G = (int)fdiv(channels, s.by_cpg);
@@ -551,11 +603,16 @@ __global__ __launch_bounds__(R > 2 ? 512 : 256, R > 4 && sizeof(T) == 2 ? 3 : 4)
     T* ob = static_cast<T*>(a.dx) + (size_t)b * a.dx_img + col.off;
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (const int nv = valid(i)) {
+        if (held.has(r + i * RT)) {
             float xh[V], dz[V];
             col.template local<SILU>(rx[i], rd[i], xh, dz, s.slope);
-            st_col<T, M>(ob + (size_t)(r + i * RT) * a.dx_row, nv, col.grad(xh, dz, s1, s2), a.past);
+            st_col<T, M>(ob + (size_t)(r + i * RT) * a.dx_row, V, col.grad(xh, dz, s1, s2), a.past);
         }
+    if (held.tail) {
+        float xh[V], dz[V];
+        col.template local<SILU>(cx, cd, xh, dz, s.slope);
+        st_col<T, M>(ob + (size_t)held.limit * a.dx_row, held.tail, col.grad(xh, dz, s1, s2), a.past);
+    }
 }
 
 // S1, S2 and the channels' sums of a chunk: x and dy read once, bound by HBM (210 MB: 40 us, 5.3 TB/s).
