@@ -5,7 +5,7 @@
 //
 // Memory bound: a value is read once, and written as one byte.  A row lives in the registers of the lanes that read it, so the
 // maximum is a few moves between lanes; with the group norm the normalised value is rounded once, to 8 bits, and no 16-bit tensor in between
-// is written or read.  12800 x 1024 fp16: 9.5 us, 16384 x 4096 bf16: 37 us (5.4 TB/s); after a group norm 204800 x 256 with silu: 37
+// is written or read.  12800 x 1024 fp16: 9 us, 16384 x 4096 bf16: 37 us (5.4 TB/s); after a group norm 204800 x 256 with silu: 37
 // us for 157 MB (4.2 TB/s), bound by memory and the vector units together (a launch that keeps those busier for fewer loads - two vectors
 // a lane - takes 38), behind the 30 us of gn_stats_kernel.
 #include "y5_common.h"
