@@ -289,11 +289,10 @@ def test_capture_beside_a_live_graph_is_refused(dev):
         want = torch.autograd.grad(alive, leaves, dy, retain_graph=True)
         torch.cuda.synchronize()
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            y = group_norm(leaves[0], 4, leaves[1], leaves[2], act='silu')
             with pytest.raises(RuntimeError, match='live graph'):
-                group_norm(leaves[0], 4, leaves[1], leaves[2], act='silu')
-            with torch.no_grad():
-                group_norm(leaves[0], 4, leaves[1], leaves[2], act='silu')
-        del alive
+                torch.autograd.grad(y, leaves, dy)
+        del alive, y
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             got = torch.autograd.grad(group_norm(leaves[0], 4, leaves[1], leaves[2], act='silu'), leaves, dy)

@@ -104,19 +104,19 @@ Tensor run_forward(const Tensor& x, const Norm& n, const Tensor& weight, const T
 }
 
 // torch keeps one accumulation node a leaf as long as any graph of it lives, on the stream of the first.  The default stream cannot
-// join a capture: the captured gradient of a leaf whose node lives there ends the process, so its forward pass is refused.
-void check_leaf(const Tensor& t, const char* name) {
-    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
+// join a capture: the captured gradient of a leaf whose node lives there ends the process.  Under capture the forward pass looks for
+// such leaves (the node would otherwise be made with this call's own), and the gradient is refused.
+bool lives_elsewhere(const Tensor& t) {
+    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return false;
     const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-    if (!node) return;
+    if (!node) return false;
     const auto stream = node->stream();
-    TORCH_CHECK(!stream || stream->id() != c10::hip::getDefaultHIPStream(t.get_device()).id(), "group_norm: ", name,
-                " has a live graph on the default stream, which its captured gradient would have to wait for: drop that graph before the capture");
+    return stream && stream->id() == c10::hip::getDefaultHIPStream(t.get_device()).id();
 }
 
 struct GroupNorm : torch::autograd::Function<GroupNorm> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, Maybe weight, Maybe bias, int64_t pitch, int64_t groups, double eps,
-                          int64_t act, double slope) {
+                          int64_t act, double slope, bool refused) {
         const Tensor w = or_none(weight), b = or_none(bias);
         const Tensor stats = at::empty({2, x.size(0), groups}, x.options().dtype(at::kFloat));  // mean and 1 / deviation
         const Tensor y = run_forward(x, Norm{pitch, groups, act, eps, slope}, w, b, stats);
@@ -126,6 +126,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
         ctx->saved_data["act"] = act;
         ctx->saved_data["eps"] = eps;
         ctx->saved_data["slope"] = slope;
+        ctx->saved_data["refused"] = refused;
         return y;
     }
 
@@ -133,6 +134,8 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &stats = saved[3];
         auto& kept = ctx->saved_data;
+        TORCH_CHECK(!kept["refused"].toBool(), "group_norm: a live graph on the default stream holds x, weight or bias, and their captured gradient would have to wait "
+                                               "for that stream: drop the graph before the capture");
         const Norm n{kept["pitch"].toInt(), kept["groups"].toInt(), kept["act"].toInt(), kept["eps"].toDouble(), kept["slope"].toDouble()};
         Tensor dx, dw, db;
         {
@@ -162,19 +165,16 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
             for (Tensor* t : {&dx, &dw, &db})
                 if (t->defined()) *t = out[i++];
         }
-        return {dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        return {dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 
 Tensor group_norm(const Tensor& x, int64_t pitch, int64_t groups, Maybe weight, Maybe bias, double eps, int64_t act, double slope) {
     const Tensor w = or_none(weight), b = or_none(bias);
     if (at::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()))) {
-        if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
-            check_leaf(x, "x");
-            check_leaf(w, "weight");
-            check_leaf(b, "bias");
-        }
-        return GroupNorm::apply(x, weight, bias, pitch, groups, eps, act, slope);
+        const bool refused = c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None &&
+                             (lives_elsewhere(x) || lives_elsewhere(w) || lives_elsewhere(b));
+        return GroupNorm::apply(x, weight, bias, pitch, groups, eps, act, slope, refused);
     }
     return run_forward(x, Norm{pitch, groups, act, eps, slope}, w, b, Tensor());
 }

@@ -100,8 +100,8 @@ def _plain(x, num_groups, weight, bias, eps, act, slope):
 def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, act=None, slope=0.1):
     """act(group_norm(x)) in x's type, channels_last.  weight, bias: (channels,) of one type (x's, or fp32 beside a 16-bit x),
     or None.  act: None, 'leaky' (with slope) or 'silu'.  Differentiable once in x, weight and bias; their gradients
-    come in their own types, each sum rounded once.  Under graph capture, leaves of which a graph made on the default stream
-    still lives are refused (the captured gradient could not be accumulated)."""
+    come in their own types, each sum rounded once.  A captured gradient is refused for leaves of which a graph made on the
+    default stream still lives: torch would have it wait for that stream."""
     _check(x, num_groups, weight, bias, eps, act)
     if not x.is_cuda or x.numel() == 0:
         return _plain(x, num_groups, weight, bias, eps, act, slope)
