@@ -816,9 +816,11 @@ int run_rows(const NormShape& s, int esize) {
     return rows < 1 ? 1 : (int)rows;
 }
 
-// Bytes of a slice that few workgroups (below 128) may hold all the same: a larger one is read by a few compute units while the others idle
-// (3 x 45 x 27 x 75 fp16, 182 KB: 28 us, split 14; 40 x 40 x 64 in one group, 205 KB: 18 against 9; 2 x 20 x 20 x 128, 102 KB: 12.7 against 8.9;
-// 20 x 20 x 64, 51 KB: the same; the other way round only 64 images of 20 x 20 x 255, 204 KB: 30 against 45).
+// Bytes of a slice that few workgroups (below 64; below 128 four times of it) may hold all the same: a larger one is read by a few compute
+// units while the others idle.  With 64 to 127 workgroups 2 x 40 x 40 x 512, 51 KB, resident 9.5 us (fp32 11), split 13 (17);
+// 2 x 20 x 20 x 1024 fp32 7.2, split 12; 64 x 40 x 40 x 64 in one group, 205 KB, 21, split 18.  Below 64 it depends: 20 x 20 x 1024 fp32
+// 7.1, split 11, but the gradient of 60 x 60 x 256 fp16 30 with the forward, split 24, and 3 x 45 x 27 x 75 fp16, 182 KB, 28, split 14.
+// Images of odd channel counts, whose split form has more to set up, have no second bound (64 x 20 x 20 x 255, 204 KB: 30, split 45).
 constexpr int kResidentAlone = 32 << 10;
 constexpr long long kCache = 256 << 20;  // bytes of the cache in front of HBM
 
@@ -858,7 +860,7 @@ bool resident_of(const NormShape& s, int esize, bool bwd, Resident* out) {
             while (cols * 16 < width && s.cols % (cols * 2) == 0 && (long long)s.batch * (s.cols / (cols * 2)) >= 256) cols *= 2;
         }
         const long long wgs = (long long)s.batch * (s.cols / cols), bytes = (long long)s.vrows * cols * 16;
-        if (bytes > kResidentAlone && wgs < 128) return false;
+        if ((bytes > kResidentAlone && wgs < 64) || (s.k == 1 && bytes > 4 * kResidentAlone && wgs < 128)) return false;
         if (!bwd) {
             if (resident_fit(s, cols, kFwdCap, out)) return true;
         } else if (resident_fit(s, cols, kBwdCap, out)) {
